@@ -1181,6 +1181,170 @@ def attention(q, kt, v, mask=None, scale=1.0):
     return Attention(scale)(*args)[0]
 
 
+class Rotary(Operator):
+    """Rotary positions of the heads of x (batch, sequence, heads, head_dim),
+    or of queries and keys with head counts of their own in one launch:
+
+        Rotary(handle, positions)(x)                      -> (y,)
+        Rotary(handle, positions)(q, k)                   -> (q', k')
+        Rotary(handle, positions, norm=True)(q, k, wq, wk) -> (q', k')
+
+    With ``norm`` every head is first divided by its root mean square and
+    multiplied by its scale (head_dim,): x / sqrt(mean(x^2) + eps) * w.
+    ``handle`` is a ``RotaryHandle``; ``positions`` an int32 Tensor
+    (sequence,) or (batch, sequence) -- a server's single tokens, packed
+    sequences that begin again -- or None for 0 .. sequence - 1.  Strided
+    views (a transposed (batch, heads, sequence, head_dim)) are read in place;
+    the outputs are contiguous."""
+
+    def __init__(self, handle, positions=None, norm=False, eps=1e-6):
+        super(Rotary, self).__init__()
+        self.handle, self.norm, self.eps = handle, bool(norm), float(eps)
+        self.positions = None if positions is None else positions.data
+
+    def forward(self, *xs):
+        if self.norm and (len(xs) % 2 or not xs):
+            raise ValueError("a normed rotary takes a scale for each tensor")
+        n = len(xs) // 2 if self.norm else len(xs)
+        if training:
+            self.inputs = xs
+        ys = singa.RotaryForward(self.handle, xs[:n], xs[n:], self.positions,
+                                 self.eps)
+        return tuple(ys)
+
+    def backward(self, *dys):
+        n = len(self.inputs) // 2 if self.norm else len(self.inputs)
+        xs, scales = self.inputs[:n], self.inputs[n:]
+        # an output that nothing uses has no gradient
+        dys = [_scalar_like(x, 0.0) if dy is None else dy
+               for x, dy in zip(xs, dys)]
+        dxs, dws = singa.RotaryBackward(self.handle, dys, xs, scales,
+                                        self.positions, self.eps)
+        return tuple(dxs) + tuple(dws)
+
+
+def rotary(handle, x, positions=None, scale=None, eps=1e-6):
+    """Rotary positions of one tensor, after its norm when it has a scale."""
+    args = (x,) if scale is None else (x, scale)
+    return Rotary(handle, positions, scale is not None, eps)(*args)[0]
+
+
+def rotary_qk(handle, q, k, positions=None, q_scale=None, k_scale=None,
+              eps=1e-6):
+    """Rotary positions of queries and keys in one launch, after the norm of
+    their heads when they have scales (both or neither)."""
+    if (q_scale is None) != (k_scale is None):
+        raise ValueError("both scales or neither")
+    args = (q, k) if q_scale is None else (q, k, q_scale, k_scale)
+    return Rotary(handle, positions, q_scale is not None, eps)(*args)
+
+
+class _TokenLoss(Operator):
+    """A loss over log p(t) = x[t] - log sum exp(x) of the labels t (int32, the
+    logits' shape without its last dimension).  A label outside the vocabulary
+    (padding, a prompt: -1) takes no part: its logits are not read, its
+    gradient is zero.  Results are float32 whatever the logits' type.  The
+    logits are read once forward and once backward; nothing of their size but
+    the gradient is written."""
+
+    def __init__(self, t):
+        super(_TokenLoss, self).__init__()
+        self.t = t.data
+
+    def _loss(self, x):
+        raise NotImplementedError
+
+    def forward(self, x):
+        loss = self._loss(x)
+        y = loss.forward()
+        if training:
+            self.loss = loss
+        return y
+
+    def backward(self, dy=1.0):
+        return self.loss.backward(dy)
+
+
+class TokenLogProb(_TokenLoss):
+    """The log-probability of every label, (labels' shape); 0 where the label
+    is ignored."""
+
+    def _loss(self, x):
+        return singa.TokenLoss(singa.LOSS_LOG_PROB, x, self.t)
+
+
+def token_log_prob(x, t):
+    return TokenLogProb(t)(x)[0]
+
+
+class PreferenceLoss(_TokenLoss):
+    """Paired log-ratio loss over 2 P sequences, the P chosen ones first and
+    then the P rejected ones in the same order.  With a_i the sum over
+    sequence i of log p(t) - reference,
+
+        z = beta (a_chosen - a_rejected)
+        loss = -mean((1 - smoothing) log sigma(z) + smoothing log sigma(-z))
+
+    x (2 P, S, V), t and reference (2 P, S); ``reference`` are the frozen
+    model's log-probabilities, as ``token_log_prob`` gives them."""
+    takes_scalar_dy = True
+
+    def __init__(self, t, reference, beta=0.1, smoothing=0.0):
+        super(PreferenceLoss, self).__init__(t)
+        if not 0.0 <= smoothing <= 1.0:
+            raise ValueError("smoothing is from 0 to 1, got %r" % (smoothing,))
+        self.reference = reference.data
+        self.beta, self.smoothing = float(beta), float(smoothing)
+
+    def _loss(self, x):
+        return singa.TokenLoss(singa.LOSS_PREFERENCE, x, self.t,
+                               ref=self.reference, beta=self.beta,
+                               smoothing=self.smoothing)
+
+
+def preference_loss(x, t, reference, beta=0.1, smoothing=0.0):
+    return PreferenceLoss(t, reference, beta, smoothing)(x)[0]
+
+
+class PolicyLoss(_TokenLoss):
+    """Clipped policy loss with a divergence term, over all tokens that take
+    part:
+
+        r = exp(log p(t) - old),  d = reference - log p(t)
+        loss = sum w (-min(r A, clip(r, 1 - clip[0], 1 + clip[1]) A)
+                      + kl (exp(d) - d - 1)) / sum w
+
+    old (the sampling policy's log-probabilities), advantages, weights (1
+    without; a token of weight 0 takes no part) and reference (no divergence
+    term without) have the labels' shape.  0 when the weights that take part
+    add up to 0."""
+    takes_scalar_dy = True
+
+    def __init__(self, t, old, advantages, weights=None, reference=None,
+                 clip=(0.2, 0.2), kl=0.0):
+        super(PolicyLoss, self).__init__(t)
+        low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
+        if not (0.0 <= low <= 1.0 and high >= 0.0):
+            raise ValueError("clip is (0 to 1, from 0), got %r" % (clip,))
+        if kl and reference is None:
+            raise ValueError("a divergence term needs reference "
+                             "log-probabilities")
+        self.given = [None if a is None else a.data
+                      for a in (old, advantages, weights, reference)]
+        self.clip, self.kl = (float(low), float(high)), float(kl)
+
+    def _loss(self, x):
+        old, adv, weight, ref = self.given
+        return singa.TokenLoss(singa.LOSS_POLICY, x, self.t,
+                               ref=ref if self.kl else None, old=old, adv=adv,
+                               weight=weight, clip=self.clip, kl=self.kl)
+
+
+def policy_loss(x, t, old, advantages, weights=None, reference=None,
+                clip=(0.2, 0.2), kl=0.0):
+    return PolicyLoss(t, old, advantages, weights, reference, clip, kl)(x)[0]
+
+
 class BinaryCrossEntropy(Operator):
     """-mean_batch sum(t log(x + eps) + (1 - t) log(1 - x + eps))."""
     takes_scalar_dy = True

@@ -11,6 +11,7 @@ primitives every backend must provide) and tensor_math_cpp.h.
 """
 import math
 
+import numpy as np
 import torch
 import torch.nn.functional as F
 
@@ -38,6 +39,48 @@ _BINARY = {
     # dy where x > 0 else 0  (operands: dy, x)
     "relu_bwd": lambda dy, x: dy * (x > 0).to(dy.dtype),
 }
+
+
+# ---- 8-bit optimizer states: e4m3 codes, four to an int32 word, and one float
+# scale for each 256 of them ----
+def _from_codes(words, scales):
+    codes = words.view(torch.uint8).view(torch.float8_e4m3fn).float()
+    return (codes.view(-1, 256) * scales.view(-1, 1)).view(-1)
+
+
+def _to_codes(x, noise, words, scales, keep):
+    """Codes and scales of x; ``noise`` (16 bits for each) decides the
+    rounding.  keep: what is positive does not become zero."""
+    x = F.pad(x, (0, 4 * words.numel() - x.numel())).view(-1, 256)
+    size = x.abs()
+    top = torch.where(size.isfinite(), size, 0.0).amax(1, keepdim=True)
+    top = torch.where(top > 2.0 ** -110, top, 0.0)
+    t = x * torch.where(top > 0, 448.0 / top, 0.0)
+    size = t.abs()
+    power = (torch.frexp(size.clamp_min(2.0 ** -6)).exponent - 4).float()
+    unit = torch.exp2(power)
+    q = torch.floor(size / unit + noise.view(-1, 256).float() / 65536) * unit
+    if keep:
+        q = torch.where(size > 0, q.clamp_min(2.0 ** -9), q)
+    q = torch.copysign(torch.where(x.isfinite(), q.clamp_max(448.0),
+                                   float("nan")), t)
+    words.copy_(q.view(-1).to(torch.float8_e4m3fn).view(torch.uint8)
+                .view(torch.int32))
+    scales.copy_(top.view(-1) / 448.0)
+
+
+def _philox_words(groups, step, seed):
+    """Philox4x32-10 of the counters (0 .. groups - 1, step): 4 words each."""
+    low = 0xffffffff
+    i = torch.arange(groups)
+    c = [i & low, i >> 32, torch.full_like(i, step), torch.zeros_like(i)]
+    k = [seed & low, seed >> 32 & low]
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57    # 64 bits, wrapping
+        c = [(b >> 32 & low) ^ c[1] ^ k[0], b & low,
+             (a >> 32 & low) ^ c[3] ^ k[1], a & low]
+        k = [k[0] + 0x9E3779B9 & low, k[1] + 0xBB67AE85 & low]
+    return torch.stack(c, -1).view(-1)
 
 
 class CpuMath(object):
@@ -430,6 +473,156 @@ class CpuMath(object):
                                               eps)
             s1[i].copy_(u)
             p.copy_(pv - lr * upd)
+
+    # ---- AdamW (same contract as the HIP backend) --------------------------------
+    def adamw_update_multi(self, sizes, ps, gs, masters, s1, s2, sc1, sc2, lr,
+                           wd, eps, b1, b2, step, state_bits, scale, seed):
+        one = np.float32(1.0)
+        lr, wd, eps, b1, b2 = (np.float32(t.reshape(-1)[0].item())
+                               for t in (lr, wd, eps, b1, b2))
+        step = int(step.reshape(-1)[0].item())
+        # 1 - b^t from 1 - b as float32 holds it
+        c1, c2 = (float(-np.expm1((step + 1) * np.log1p(-np.float64(one - b))))
+                  for b in (b1, b2))
+        k1, k2, decay = float(one - b1), float(one - b2), float(lr * wd)
+        lr, eps, b1, b2 = float(lr), float(eps), float(b1), float(b2)
+        for i, n in enumerate(sizes):
+            p = masters[i] if masters else ps[i]
+            g = gs[i][:n].float() * scale
+            if state_bits == 32:
+                m, v = s1[i][:n], s2[i][:n]
+            else:
+                m = _from_codes(s1[i], sc1[i])[:n]
+                v = _from_codes(s2[i], sc2[i])[:n].square()
+            m = b1 * m + k1 * g
+            v = b2 * v + k2 * (g * g)
+            q = p[:n].float()
+            q = q - decay * q
+            q = q - lr * ((m / c1) / (torch.sqrt(v / c2) + eps))
+            p[:n].copy_(q)
+            if masters:
+                ps[i][:n].copy_(q)
+            if state_bits == 32:
+                s1[i][:n].copy_(m)
+                s2[i][:n].copy_(v)
+            else:
+                noise = _philox_words(-(-n // 256) * 64, step, seed)
+                _to_codes(m, noise & 0xffff, s1[i], sc1[i], False)
+                _to_codes(torch.sqrt(v), noise >> 16, s2[i], sc2[i], True)
+
+    # ---- rotary positions ---------------------------------------------------------
+    def rotary(self, handle, xs, dys, ws, pos, ys, dws, eps):
+        B, S = ys[0].shape[:2]
+        R, half = handle.rotary_dim, handle.layout == "half"
+        at = torch.arange(S) if pos is None else pos
+        angle = at.double().unsqueeze(-1) * torch.from_numpy(handle.frequencies)
+        cos = (handle.amplitude * torch.cos(angle)).unsqueeze(-2)
+        sin = (handle.amplitude * torch.sin(angle)).unsqueeze(-2)
+
+        def turn(x, sin):
+            y = x.clone()
+            first = slice(0, R // 2) if half else slice(0, R, 2)
+            second = slice(R // 2, R) if half else slice(1, R, 2)
+            a, b = x[..., first], x[..., second]
+            y[..., first] = a * cos - b * sin
+            y[..., second] = a * sin + b * cos
+            return y
+
+        for i, y in enumerate(ys):
+            if ws:
+                w = ws[i].double()
+                x = xs[i].double()
+                rstd = 1.0 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+                xh = x * rstd
+            if not dys:
+                y.copy_(turn(xh * w if ws else xs[i].double(), sin))
+                continue
+            g = turn(dys[i].double(), -sin)
+            if ws:
+                dws[i].copy_((g * xh).sum((0, 1, 2)))
+                g = g * w
+                g = rstd * (g - xh * (g * xh).mean(-1, keepdim=True))
+            y.copy_(g)
+
+    # ---- losses over token log-probabilities ------------------------------------------
+    @staticmethod
+    def _token_rows(mode, x, label, rows, V, weight):
+        label = label[:rows]
+        used = (label >= 0) & (label < V)
+        if mode == 2 and weight is not None:
+            used = used & (weight[:rows] != 0)
+        return used, torch.where(used, label, 0).long().unsqueeze(-1)
+
+    def token_loss_fwd(self, spec, x, label, extra, value, saved, loss):
+        mode, rows, V, pairs, seq, consts = spec
+        beta, smooth, lo, hi, kl = consts
+        ref, old, adv, weight = [None if t is None else t[:rows].double()
+                                 for t in extra]
+        used, at = self._token_rows(mode, x, label, rows, V, weight)
+        x = x[:rows * V].view(rows, V).double()
+        top = x.amax(-1, keepdim=True)
+        norm = torch.log(torch.exp(x - top).sum(-1, keepdim=True))
+        lp = ((x.gather(-1, at) - top) - norm).squeeze(-1)
+        zero = torch.zeros_like(lp)
+        for i, kept in enumerate((top, norm)):
+            saved[i * rows:(i + 1) * rows].copy_(
+                torch.where(used, kept.squeeze(-1), zero))
+        saved = saved[2 * rows:]
+        if mode == 0:
+            value[:rows].copy_(torch.where(used, lp, zero))
+        elif mode == 1:
+            each = torch.where(used, lp - ref, zero)
+            value[:rows].copy_(each)
+            side = each.view(2, pairs, seq).sum(-1)
+            z = beta * (side[0] - side[1])
+            loss.copy_(((1 - smooth) * F.softplus(-z) +
+                        smooth * F.softplus(z)).mean())
+            saved[:pairs].copy_(
+                (smooth * torch.sigmoid(z) -
+                 (1 - smooth) * torch.sigmoid(-z)) * beta / pairs)
+        else:
+            w = torch.ones_like(lp) if weight is None else weight
+            w = torch.where(used, w, zero)
+            ratio = torch.exp(lp - old)
+            plain, cut = ratio * adv, ratio.clamp(lo, hi) * adv
+            clipped = cut < plain
+            each = -torch.where(clipped, cut, plain)
+            c = torch.where(clipped, zero, -plain)
+            if ref is not None:
+                d = ref - lp
+                each = each + kl * (torch.expm1(d) - d)
+                c = c - kl * torch.expm1(d)
+            each = torch.where(used, w * each, zero)
+            value[:rows].copy_(each)
+            total = w.sum()
+            total = total if float(total) > 0 else torch.ones_like(total)
+            loss.copy_(each.sum() / total)
+            saved[:rows].copy_(torch.where(used, w * c, zero))
+            saved[rows:rows + 1].copy_(1.0 / total)
+
+    def token_loss_bwd(self, spec, x, label, saved, weight, dy, dy_scale, dx):
+        mode, rows, V, pairs, seq = spec
+        used, at = self._token_rows(mode, x, label, rows, V, weight)
+        top, norm = saved[:2 * rows].double().view(2, rows, 1)
+        saved = saved[2 * rows:]
+        if mode == 0:
+            c = dy[:rows].double()
+        else:
+            c = torch.full((rows,), dy_scale, dtype=torch.float64)
+            if dy is not None:
+                c = c * dy.double()[0]
+            if mode == 1:
+                dz = saved[:pairs].double()
+                c = c * torch.cat([dz, -dz]).repeat_interleave(seq)
+            else:
+                c = c * saved[:rows].double() * saved[rows].double()
+        used = used & (c != 0)
+        c = torch.where(used, c, torch.zeros_like(c)).unsqueeze(-1)
+        x = x[:rows * V].view(rows, V).double()
+        g = -c * torch.exp((x - top) - norm)
+        g.scatter_add_(-1, at, c)
+        g = torch.where(used.unsqueeze(-1), g, torch.zeros_like(g))
+        dx[:rows * V].view(rows, V).copy_(g)
 
     # ---- fused attention (same contract as the HIP backend) ------------------------
     @staticmethod

@@ -11,6 +11,7 @@ the graph's private pool).
 Contract parity: reference src/core/tensor/tensor_math.h:86-485 and
 tensor_math_cuda.h (the CUDA specialisations this backend stands in for).
 """
+import contextlib
 import json
 import math
 import os
@@ -125,6 +126,9 @@ _COLS_SCRATCH = 1 << 16
 _CONV_SIDE_ZERO = os.environ.get("SINGA_CONV_SIDE_ZERO", "1") != "0"
 _CONV3X3_GEMM_MIN_HW = int(os.environ.get("SINGA_CONV3X3_GEMM_MIN_HW", "2000"))
 
+_NOTHING = contextlib.nullcontext()
+
+
 def _raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
@@ -179,6 +183,13 @@ class HipMath(object):
         # raw handle of the current stream of this device (follows stream
         # contexts and graph capture) without building a Stream object
         return _raw_stream(self._dev_index)
+
+    def _current(self):
+        """Context in which this device is the current one: a launch goes to
+        the current device, whatever device its stream belongs to."""
+        if torch._C._cuda_getDevice() == self._dev_index:
+            return _NOTHING
+        return torch.cuda.device(self._dev_index)
 
     def _tmp(self, n, dtype=torch.float32):
         return torch.empty(n, dtype=dtype, device=self.dev.torch_device)
@@ -1754,6 +1765,81 @@ class HipMath(object):
             [t.data_ptr() for t in s2] if s2 else [],
             [p.numel() for p in ps], ptr[0], ptr[1], ptr[2], ptr[3], ptr[4],
             ptr[5], float(scale), self._s())
+
+    def adamw_update_multi(self, sizes, ps, gs, masters, s1, s2, sc1, sc2, lr,
+                           wd, eps, b1, b2, step, state_bits, scale, seed):
+        """One AdamW step on a list of flat parameters of one type, one launch
+        per 48 tensors (see lm_ops.AdamWUpdateMulti)."""
+        def ptrs(ts):
+            return [t.data_ptr() for t in ts]
+
+        with self._current():
+            self.k.adamw_update_multi(
+                _code(ps[0]), state_bits, ptrs(ps), ptrs(gs), ptrs(masters),
+                ptrs(s1), ptrs(s2), ptrs(sc1), ptrs(sc2), sizes, lr.data_ptr(),
+                wd.data_ptr(), eps.data_ptr(), b1.data_ptr(), b2.data_ptr(),
+                step.data_ptr(), scale, seed & 0xffffffffffffffff, self._s())
+
+    # ---- rotary positions ---------------------------------------------------------
+    def rotary(self, handle, xs, dys, ws, pos, ys, dws, eps):
+        """Forward without ``dys``, else backward: xs (empty for a rotation
+        alone) and dys (B, S, H, D) views with a contiguous last dimension, ys
+        and dws contiguous outputs (see lm_ops.RotaryForward)."""
+        back = bool(dys)
+        B, S, _, D = ys[0].shape
+        none = (0, 0, 0)
+        keep, parts = [], []
+        for i, y in enumerate(ys):
+            x, g = xs[i] if xs else None, dys[i] if back else None
+            part = 0
+            if dws:
+                t = self._tmp(self.k.ROTARY_MAX_BLOCKS * D)
+                keep.append(t)
+                part = t.data_ptr()
+            parts.append((
+                x.data_ptr() if xs else 0, g.data_ptr() if back else 0,
+                ws[i].data_ptr() if ws else 0, y.data_ptr(),
+                dws[i].data_ptr() if dws else 0, part, y.shape[2],
+                x.stride()[:3] if xs else none,
+                g.stride()[:3] if back else none))
+        at = (0, 0) if pos is None else \
+            (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
+        with self._current():
+            self.k.rotary(_code(ys[0]), back, parts,
+                          0 if pos is None else pos.data_ptr(), at, B, S, D,
+                          handle.rotary_dim, handle.layout == "half",
+                          bool(ws), eps, handle.amplitude,
+                          handle._turns.ctypes.data, self._s())
+
+    # ---- losses over token log-probabilities ------------------------------------------
+    def token_loss_fwd(self, spec, x, label, extra, value, saved, loss):
+        """lm_ops.TokenLoss.forward on flat operands."""
+        mode, rows, V, pairs, seq, consts = spec
+        saved_at = saved.data_ptr()
+        pieces = self.k.token_loss_pieces(rows, V)
+        part = self._tmp(2 * rows * pieces) if pieces > 1 else None
+        sums = self._tmp(2 * pairs, torch.float64) if pairs else None
+        at = (saved_at, saved_at + 4 * rows, value.data_ptr(),
+              saved_at + 8 * rows, saved_at + (12 if mode == 2 else 8) * rows,
+              sums.data_ptr() if pairs else 0,
+              part.data_ptr() if pieces > 1 else 0)
+        with self._current():
+            self.k.token_loss_fwd(
+                _code(x), mode, x.data_ptr(), label.data_ptr(), rows, V, pairs,
+                seq, *[0 if t is None else t.data_ptr() for t in extra],
+                consts, at, 0 if loss is None else loss.data_ptr(), self._s())
+
+    def token_loss_bwd(self, spec, x, label, saved, weight, dy, dy_scale, dx):
+        mode, rows, V, pairs, seq = spec
+        at = saved.data_ptr()
+        with self._current():
+            self.k.token_loss_bwd(
+                _code(x), mode, x.data_ptr(), label.data_ptr(), rows, V, pairs,
+                seq, 0 if weight is None else weight.data_ptr(), at,
+                at + 4 * rows, at + 8 * rows,
+                at + (12 if mode == 2 else 8) * rows,
+                0 if dy is None else dy.data_ptr(), dy_scale, dx.data_ptr(),
+                self._s())
 
     # ---- layer norm / gelu ------------------------------------------------------
     def layernorm_fwd(self, x, gamma, beta, y, mean, rstd, eps):

@@ -5,14 +5,21 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <array>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "kernels.h"
 
 namespace py = pybind11;
+using sa::AdamwHyper;
 using sa::Desc;
+using sa::kRotaryMaxBlocks;
+using sa::RotaryDesc;
+using sa::RotaryTensor;
+using sa::TokenLossDesc;
 
 namespace {
 
@@ -770,6 +777,125 @@ PYBIND11_MODULE(_hip, m) {
               (const float *)CP(eps), (const float *)CP(a),
               (const float *)CP(b), (const float *)CP(step), scale, S(s)),
           "adaptive_update_multi");
+  });
+
+  m.def("adamw_update_multi", [](int dt, int state_bits,
+                                 std::vector<uintptr_t> p,
+                                 std::vector<uintptr_t> g,
+                                 std::vector<uintptr_t> master,
+                                 std::vector<uintptr_t> mm,
+                                 std::vector<uintptr_t> vv,
+                                 std::vector<uintptr_t> ms,
+                                 std::vector<uintptr_t> vs,
+                                 std::vector<int64_t> n, uintptr_t lr,
+                                 uintptr_t wd, uintptr_t eps, uintptr_t b1,
+                                 uintptr_t b2, uintptr_t step, float scale,
+                                 uint64_t seed, uintptr_t s) {
+    const size_t k = p.size();
+    auto of = [&](size_t have, bool needed) {
+      return have == k || (have == 0 && !needed);
+    };
+    const bool eight = state_bits == 8;
+    if (!of(g.size(), true) || !of(master.size(), false) ||
+        !of(mm.size(), true) || !of(vv.size(), true) || !of(ms.size(), eight) ||
+        !of(vs.size(), eight) || !of(n.size(), true))
+      throw std::invalid_argument("adamw_update_multi: list lengths differ");
+    const AdamwHyper h{(const float *)CP(lr),  (const float *)CP(wd),
+                       (const float *)CP(eps), (const float *)CP(b1),
+                       (const float *)CP(b2),  (const float *)CP(step),
+                       scale,                  seed};
+    auto floats = [](std::vector<uintptr_t> &a) {
+      return a.empty() ? nullptr : reinterpret_cast<float *const *>(a.data());
+    };
+    check(sa_adamw_update_multi(
+              dt, state_bits, (int)k, reinterpret_cast<void *const *>(p.data()),
+              reinterpret_cast<const void *const *>(g.data()), floats(master),
+              reinterpret_cast<void *const *>(mm.data()),
+              reinterpret_cast<void *const *>(vv.data()), floats(ms),
+              floats(vs), n.data(), &h, S(s)),
+          "adamw_update_multi");
+  });
+
+  // ---- rotary positions ------------------------------------------------------
+  // parts: one (x, dy, w, y, dw, partial, H, 3 strides of x, 3 of dy) for each
+  // tensor; freq: address of R / 2 host words
+  using RotaryPartTuple =
+      std::tuple<uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t,
+                 uintptr_t, int, std::array<int64_t, 3>,
+                 std::array<int64_t, 3>>;
+  m.attr("ROTARY_MAX_BLOCKS") = kRotaryMaxBlocks;
+  m.def("rotary", [](int dt, bool backward, std::vector<RotaryPartTuple> parts,
+                     uintptr_t pos, std::array<int64_t, 2> pos_stride,
+                     int64_t B, int64_t S_, int D, int R, bool half, bool norm,
+                     float eps, float amplitude, uintptr_t freq, uintptr_t s) {
+    if (parts.empty() || parts.size() > 2)
+      throw std::invalid_argument("rotary: one or two tensors");
+    RotaryDesc d;
+    d.parts = (int)parts.size();
+    for (int i = 0; i < d.parts; ++i) {
+      RotaryTensor &t = d.part[i];
+      const RotaryPartTuple &q = parts[i];
+      t.x = CP(std::get<0>(q));
+      t.dy = CP(std::get<1>(q));
+      t.w = CP(std::get<2>(q));
+      t.y = P(std::get<3>(q));
+      t.dw = P(std::get<4>(q));
+      t.partial = (float *)P(std::get<5>(q));
+      t.H = std::get<6>(q);
+      for (int k = 0; k < 3; ++k) {
+        t.x_stride[k] = std::get<7>(q)[k];
+        t.dy_stride[k] = std::get<8>(q)[k];
+      }
+    }
+    d.pos = (const int *)CP(pos);
+    d.pos_stride[0] = pos_stride[0];
+    d.pos_stride[1] = pos_stride[1];
+    d.B = B; d.S = S_; d.D = D; d.R = R; d.half = half; d.norm = norm;
+    d.eps = eps; d.amplitude = amplitude;
+    d.freq = reinterpret_cast<const uint64_t *>(freq);
+    check(backward ? sa_rotary_bwd(dt, &d, S(s)) : sa_rotary_fwd(dt, &d, S(s)),
+          "rotary");
+  });
+
+  // ---- losses over token log-probabilities -------------------------------------
+  m.def("token_loss_pieces", &sa_token_loss_pieces);
+  // saved: (top, norm, value, coef, total, seq_sum, part) addresses
+  m.def("token_loss_fwd", [](int dt, int mode, uintptr_t x, uintptr_t label,
+                             int64_t rows, int64_t V, int64_t pairs,
+                             int64_t seq, uintptr_t ref, uintptr_t old,
+                             uintptr_t adv, uintptr_t weight,
+                             std::array<float, 5> consts,
+                             std::array<uintptr_t, 7> saved, uintptr_t loss,
+                             uintptr_t s) {
+    TokenLossDesc d;
+    d.mode = mode; d.x = CP(x); d.label = (const int *)CP(label);
+    d.rows = rows; d.V = V; d.pairs = pairs; d.seq = seq;
+    d.ref = (const float *)CP(ref); d.old = (const float *)CP(old);
+    d.adv = (const float *)CP(adv); d.weight = (const float *)CP(weight);
+    d.beta = consts[0]; d.smoothing = consts[1]; d.clip_lo = consts[2];
+    d.clip_hi = consts[3]; d.kl = consts[4];
+    d.top = (float *)P(saved[0]); d.norm = (float *)P(saved[1]);
+    d.value = (float *)P(saved[2]); d.coef = (float *)P(saved[3]);
+    d.total = (float *)P(saved[4]); d.seq_sum = (double *)P(saved[5]);
+    d.part = (float2 *)P(saved[6]);
+    d.loss = (float *)P(loss);
+    check(sa_token_loss_fwd(dt, &d, S(s)), "token_loss_fwd");
+  });
+  m.def("token_loss_bwd", [](int dt, int mode, uintptr_t x, uintptr_t label,
+                             int64_t rows, int64_t V, int64_t pairs,
+                             int64_t seq, uintptr_t weight, uintptr_t top,
+                             uintptr_t norm, uintptr_t coef, uintptr_t total,
+                             uintptr_t dy,
+                             float dy_scale, uintptr_t dx, uintptr_t s) {
+    TokenLossDesc d;
+    d.mode = mode; d.x = CP(x); d.label = (const int *)CP(label);
+    d.rows = rows; d.V = V; d.pairs = pairs; d.seq = seq;
+    d.weight = (const float *)CP(weight);
+    d.top = (float *)P(top); d.norm = (float *)P(norm);
+    d.coef = (float *)P(coef);
+    d.total = (float *)P(total);
+    d.dy = (const float *)CP(dy); d.dy_scale = dy_scale; d.dx = P(dx);
+    check(sa_token_loss_bwd(dt, &d, S(s)), "token_loss_bwd");
   });
 
   // ---- recurrent cells and the persistent LSTM ----------------------------------------------------------

@@ -1,0 +1,356 @@
+// AdamW (Adam with decoupled weight decay) over many tensors in one launch,
+// with the two moments in float32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2       t = step + 1
+//   p = p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// A 16-bit parameter has a float32 master that is stepped and rounded into it.
+//
+// 8-bit states: every 256 values of a tensor share one float scale per moment,
+// their largest magnitude / 448; m and r = sqrt(v) -- whose range is half that
+// of v in powers of two -- are e4m3 codes, four to a word.
+//  * Rounding is stochastic.  A step moves v by a thousandth of itself while
+//    neighbouring codes are 6 to 12 % apart: rounded to the nearest, v would
+//    never move.  floor(x + u) with uniform u keeps the expectation.  u are 16
+//    bits of Philox4x32-10 with the counter (element / 4, step) and the seed as
+//    key: a function of seed, step and place, the same on every run.
+//  * What is divided by never rounds to zero: r > 0 keeps at least the smallest
+//    code, which can only shorten a step.
+//  * A moment that is not finite is left out of its block's scale and stored as
+//    NaN: it spoils its own element, as a float32 state would, not 255 others.
+//  * The step itself uses the moments before they are rounded.
+//
+// Bound by memory: float32 reads p, g, m, v and writes p, m, v, 28 bytes an
+// element; bfloat16 with masters and 8-bit states 16 bytes.  Compiled without
+// contraction, so that a state is the same value a plain evaluation of the
+// formula in float32 gives.
+//
+// The reference has Adam only (python/singa/opt.py:608-683), one element-wise
+// launch for each operation.
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace sa {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;   // values under one scale: four for each lane
+
+struct Consts {
+  float lr, decay, eps, b1, k1, b2, k2, c1, c2, scale;
+};
+
+__device__ __forceinline__ Consts constants(const AdamwHyper &h) {
+  Consts c;
+  c.lr = h.lr[0];
+  c.decay = c.lr * h.wd[0];
+  c.eps = h.eps[0];
+  c.b1 = h.b1[0];
+  c.b2 = h.b2[0];
+  c.k1 = 1.f - c.b1;
+  c.k2 = 1.f - c.b2;
+  const float t = h.step[0] + 1.f;
+  // 1 - b^t without the cancellation of a b near 1
+  c.c1 = 1.f / -expm1f(t * log1pf(-c.k1));
+  c.c2 = 1.f / -expm1f(t * log1pf(-c.k2));
+  c.scale = h.scale;
+  return c;
+}
+
+__device__ __forceinline__ void advance(const Consts &c, float g, float &p,
+                                        float &m, float &v) {
+  g = g * c.scale;
+  m = c.b1 * m + c.k1 * g;
+  v = c.b2 * v + c.k2 * (g * g);
+  p = p - c.decay * p;
+  p = p - c.lr * ((m * c.c1) / (sqrtf(v * c.c2) + c.eps));
+}
+
+// the tensor that workgroup `chunk` works on
+__device__ __forceinline__ int tensor_of(const AdamwBatch &b, int chunk) {
+  const int lane = threadIdx.x & 63;
+  const bool behind =
+      lane > 0 && lane < b.count && chunk >= b.chunk_start[lane < b.count ? lane : 0];
+  return __popcll(__ballot(behind));
+}
+
+template <typename T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+
+template <typename T>
+__device__ __forceinline__ void load4(float *f, const T *p) {
+  const Four<T> k = *reinterpret_cast<const Four<T> *>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = to_f<T>(k.v[j]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float *f) {
+  Four<T> k;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) k.v[j] = from_f<T>(f[j]);
+  *reinterpret_cast<Four<T> *>(p) = k;
+}
+
+// four values of which the first `n` exist
+template <typename T>
+__device__ __forceinline__ void load_some(float *f, const T *p, int n,
+                                          bool wide) {
+  if (wide && n >= 4) return load4<T>(f, p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = j < n ? to_f<T>(p[j]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_some(T *p, const float *f, int n,
+                                           bool wide) {
+  if (wide && n >= 4) return store4<T>(p, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) p[j] = from_f<T>(f[j]);
+}
+
+__device__ __forceinline__ bool aligned16(const void *a, const void *b,
+                                          const void *c, const void *d,
+                                          const void *e) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+           reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d) |
+           reinterpret_cast<uintptr_t>(e)) & 15) == 0;
+}
+
+// T: type of parameter and gradient; MASTER: the step is taken on a float copy
+template <typename T, bool MASTER>
+__global__ void __launch_bounds__(kThreads)
+    adamw_kernel(AdamwBatch b, AdamwHyper h) {
+  using P = typename std::conditional<MASTER, float, T>::type;
+  const int t = tensor_of(b, blockIdx.x);
+  const int64_t base = (int64_t)((int)blockIdx.x - b.chunk_start[t]) * kAdamwChunk;
+  const int64_t left = b.n[t] - base;
+  const int len = left < kAdamwChunk ? (int)left : kAdamwChunk;
+  T *p16 = static_cast<T *>(b.p[t]) + base;
+  P *p = MASTER ? reinterpret_cast<P *>(b.master[t]) + base
+                : reinterpret_cast<P *>(p16);
+  const T *g = static_cast<const T *>(b.g[t]) + base;
+  float *m = static_cast<float *>(b.m[t]) + base;
+  float *v = static_cast<float *>(b.v[t]) + base;
+  const bool wide = aligned16(p16, p, g, m, v);
+  const Consts c = constants(h);
+  constexpr int kSteps = kAdamwChunk / (4 * kThreads);
+  float pf[kSteps][4], gf[kSteps][4], mf[kSteps][4], vf[kSteps][4];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int i = 4 * (k * kThreads + (int)threadIdx.x), n = len - i;
+    load_some<P>(pf[k], p + i, n, wide);
+    load_some<T>(gf[k], g + i, n, wide);
+    load_some<float>(mf[k], m + i, n, wide);
+    load_some<float>(vf[k], v + i, n, wide);
+  }
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int i = 4 * (k * kThreads + (int)threadIdx.x), n = len - i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      advance(c, gf[k][j], pf[k][j], mf[k][j], vf[k][j]);
+    store_some<P>(p + i, pf[k], n, wide);
+    if (MASTER) store_some<T>(p16 + i, pf[k], n, wide);
+    store_some<float>(m + i, mf[k], n, wide);
+    store_some<float>(v + i, vf[k], n, wide);
+  }
+}
+
+struct Words { uint32_t w[4]; };
+
+__device__ __forceinline__ Words philox(uint32_t c0, uint32_t c1, uint32_t c2,
+                                        uint32_t c3, uint64_t key) {
+  uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c0;
+    const uint64_t b = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return {{c0, c1, c2, c3}};
+}
+
+// the largest finite magnitude of the wave's 256 values
+__device__ __forceinline__ float block_top(const float *x) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = fabsf(x[j]);
+    top = fmaxf(top, a < INFINITY ? a : 0.f);
+  }
+  return wave_max(top);
+}
+
+// x times inv, rounded to e4m3 by the 16 bits of noise
+template <bool KEEP>
+__device__ __forceinline__ float to_code(float x, float inv, uint32_t noise) {
+  const float s = x * inv, size = fabsf(s);
+  // spacing of the codes around s: an eighth of its binade
+  const float unit =
+      __uint_as_float(__float_as_uint(fmaxf(size, 0x1p-6f)) & 0x7f800000u) *
+      0.125f;
+  float q = floorf(size / unit + (float)noise * 0x1p-16f) * unit;
+  if (KEEP) q = size > 0.f ? fmaxf(q, 0x1p-9f) : q;
+  q = q > 448.f ? 448.f : q;   // NaN stays
+  return copysignf(q, s);
+}
+
+__device__ __forceinline__ uint32_t pack_codes(const float *q) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+}
+
+__device__ __forceinline__ void unpack_codes(float *f, uint32_t w, float scale) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  f[0] = lo[0] * scale;
+  f[1] = lo[1] * scale;
+  f[2] = hi[0] * scale;
+  f[3] = hi[1] * scale;
+}
+
+// A wave takes a block of 256 values, four for each lane; the blocks of a
+// chunk go to the workgroup's four waves in turn.
+template <typename T, bool MASTER>
+__global__ void __launch_bounds__(kThreads)
+    adamw8_kernel(AdamwBatch b, AdamwHyper h) {
+  using P = typename std::conditional<MASTER, float, T>::type;
+  const int t = tensor_of(b, blockIdx.x);
+  const int64_t base = (int64_t)((int)blockIdx.x - b.chunk_start[t]) * kAdamwChunk;
+  const int64_t left = b.n[t] - base;
+  const int len = left < kAdamwChunk ? (int)left : kAdamwChunk;
+  T *p16 = static_cast<T *>(b.p[t]) + base;
+  P *p = MASTER ? reinterpret_cast<P *>(b.master[t]) + base
+                : reinterpret_cast<P *>(p16);
+  const T *g = static_cast<const T *>(b.g[t]) + base;
+  uint32_t *mw = static_cast<uint32_t *>(b.m[t]) + base / 4;
+  uint32_t *rw = static_cast<uint32_t *>(b.v[t]) + base / 4;
+  float *ms = b.m_scale[t] + base / kBlock;
+  float *rs = b.v_scale[t] + base / kBlock;
+  const bool wide = aligned16(p16, p, g, mw, rw);
+  const Consts c = constants(h);
+  const uint32_t step = (uint32_t)h.step[0];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kSteps = kAdamwChunk / (4 * kBlock);
+  float pf[kSteps][4], gf[kSteps][4], msf[kSteps], rsf[kSteps];
+  uint32_t mc[kSteps], rc[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int blk = 4 * k + wave, i = kBlock * blk + 4 * lane, n = len - i;
+    mc[k] = rc[k] = 0;
+    msf[k] = rsf[k] = 0.f;
+    if (kBlock * blk < len) {   // the last block's words are all there
+      mc[k] = mw[i / 4];
+      rc[k] = rw[i / 4];
+      msf[k] = ms[blk];
+      rsf[k] = rs[blk];
+    }
+    load_some<P>(pf[k], p + i, n, wide);
+    load_some<T>(gf[k], g + i, n, wide);
+  }
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int blk = 4 * k + wave, i = kBlock * blk + 4 * lane, n = len - i;
+    if (kBlock * blk >= len) break;   // the same for the whole wave
+    float m[4], v[4];
+    unpack_codes(m, mc[k], msf[k]);
+    unpack_codes(v, rc[k], rsf[k]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = v[j] * v[j];
+      advance(c, gf[k][j], pf[k][j], m[j], v[j]);
+      // behind the end of the tensor the states stay zero
+      m[j] = j < n ? m[j] : 0.f;
+      v[j] = j < n ? sqrtf(v[j]) : 0.f;
+    }
+    store_some<P>(p + i, pf[k], n, wide);
+    if (MASTER) store_some<T>(p16 + i, pf[k], n, wide);
+    float mt = block_top(m), rt = block_top(v);
+    // below this the reciprocal of a scale would overflow: zeros
+    mt = mt > 0x1p-110f ? mt : 0.f;
+    rt = rt > 0x1p-110f ? rt : 0.f;
+    const float mi = mt > 0.f ? 448.f * (1.f / mt) : 0.f;
+    const float ri = rt > 0.f ? 448.f * (1.f / rt) : 0.f;
+    const int64_t group = (base + i) / 4;
+    const Words u = philox((uint32_t)group, (uint32_t)((uint64_t)group >> 32),
+                           step, 0u, h.seed);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = to_code<false>(m[j], mi, u.w[j] & 0xffffu);
+      v[j] = to_code<true>(v[j], ri, u.w[j] >> 16);
+    }
+    mw[i / 4] = pack_codes(m);
+    rw[i / 4] = pack_codes(v);
+    if (lane == 0) {
+      ms[blk] = mt * (1.f / 448.f);
+      rs[blk] = rt * (1.f / 448.f);
+    }
+  }
+}
+
+template <typename T, bool MASTER>
+void launch(const AdamwBatch &b, const AdamwHyper &h, bool eight, int chunks,
+            hipStream_t s) {
+  if (eight)
+    hipLaunchKernelGGL((adamw8_kernel<T, MASTER>), dim3(chunks), dim3(kThreads),
+                       0, s, b, h);
+  else
+    hipLaunchKernelGGL((adamw_kernel<T, MASTER>), dim3(chunks), dim3(kThreads),
+                       0, s, b, h);
+}
+
+}  // namespace
+
+}  // namespace sa
+
+using namespace sa;
+
+int sa_adamw_update_multi(int dtype, int state_bits, int count, void *const *p,
+                          const void *const *g, float *const *master,
+                          void *const *m, void *const *v, float *const *m_scale,
+                          float *const *v_scale, const int64_t *n,
+                          const AdamwHyper *hyper, hipStream_t s) {
+  if (state_bits != 8 && state_bits != 32) return -2;
+  if (state_bits == 8 && (!m_scale || !v_scale)) return -2;
+  for (int first = 0; first < count;) {
+    AdamwBatch b;
+    int64_t chunks = 0;
+    int k = 0;
+    for (; k < kAdamwMaxTensors && first + k < count; ++k) {
+      const int i = first + k;
+      const int64_t mine = (n[i] + kAdamwChunk - 1) / kAdamwChunk;
+      if (mine > 0x7fffffff) return -2;
+      if (chunks + mine > 0x7fffffff) break;   // the rest in the next launch
+      b.p[k] = p[i];
+      b.g[k] = g[i];
+      b.master[k] = master ? master[i] : nullptr;
+      b.m[k] = m[i];
+      b.v[k] = v[i];
+      b.m_scale[k] = m_scale ? m_scale[i] : nullptr;
+      b.v_scale[k] = v_scale ? v_scale[i] : nullptr;
+      b.n[k] = n[i];
+      b.chunk_start[k] = (int)chunks;
+      chunks += mine;
+    }
+    b.count = k;
+    first += k;
+    if (chunks == 0) continue;
+    const bool eight = state_bits == 8;
+    SA_DISPATCH_FLOAT(dtype, T, {
+      if (master)
+        launch<T, true>(b, *hyper, eight, (int)chunks, s);
+      else
+        launch<T, false>(b, *hyper, eight, (int)chunks, s);
+    });
+  }
+  return 0;
+}

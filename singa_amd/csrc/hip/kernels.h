@@ -391,6 +391,104 @@ int sa_adaptive_update_multi(int dtype, int rule, int count, void *const *p,
                              const float *eps, const float *a, const float *b,
                              const float *step, float scale, hipStream_t s);
 
+// ---- adamw.hip ----------------------------------------------------------------
+// One AdamW step over `count` tensors in ceil(count / kAdamwMaxTensors)
+// launches; pointer arrays are host arrays, copied into the kernel arguments.
+// master: null, or a float copy of each 16-bit parameter.  state_bits 32: m and
+// v are float; 8: four e4m3 codes of m / of sqrt(v) to a word, whole blocks of
+// 256 values, with a float scale for each block.
+namespace sa {
+constexpr int kAdamwMaxTensors = 48;
+constexpr int kAdamwChunk = 4096;
+struct AdamwBatch {
+  void *p[kAdamwMaxTensors];
+  const void *g[kAdamwMaxTensors];
+  float *master[kAdamwMaxTensors];
+  void *m[kAdamwMaxTensors];
+  void *v[kAdamwMaxTensors];
+  float *m_scale[kAdamwMaxTensors];
+  float *v_scale[kAdamwMaxTensors];
+  int64_t n[kAdamwMaxTensors];
+  int chunk_start[kAdamwMaxTensors];
+  int count;
+};
+struct AdamwHyper {   // one float each in device memory; step: steps done
+  const float *lr, *wd, *eps, *b1, *b2, *step;
+  float scale;        // of the gradient
+  uint64_t seed;      // of the stochastic rounding
+};
+}  // namespace sa
+int sa_adamw_update_multi(int dtype, int state_bits, int count, void *const *p,
+                          const void *const *g, float *const *master,
+                          void *const *m, void *const *v, float *const *m_scale,
+                          float *const *v_scale, const int64_t *n,
+                          const sa::AdamwHyper *hyper, hipStream_t s);
+
+// ---- token_loss.hip ----------------------------------------------------------
+// Losses over the log-probabilities of the labels of (rows, V) logits and
+// their gradient.  float32 throughout but for the logits and their gradient.
+namespace sa {
+enum TokenLossMode : int { kLogProb = 0, kPreference = 1, kPolicy = 2 };
+struct TokenLossDesc {
+  int mode = 0;
+  const void *x = nullptr;          // (rows, V)
+  const int *label = nullptr;       // (rows); outside [0, V): ignored
+  int64_t rows = 0, V = 0;
+  int64_t pairs = 0, seq = 0;       // preference: rows = 2 pairs seq
+  const float *ref = nullptr;       // (rows); policy: may be null (no kl term)
+  const float *old = nullptr, *adv = nullptr;   // policy: (rows)
+  const float *weight = nullptr;    // policy: (rows) or null for 1
+  float beta = 0.f, smoothing = 0.f, clip_lo = 1.f, clip_hi = 1.f, kl = 0.f;
+  // (rows): maximum of the logits, log of the sum of exp(x - maximum), result
+  float *top = nullptr, *norm = nullptr, *value = nullptr;
+  float *coef = nullptr;            // policy: (rows)
+  float *total = nullptr;           // preference: (pairs), policy: (1)
+  double *seq_sum = nullptr;        // preference: (2 pairs)
+  float *loss = nullptr;            // (1)
+  float2 *part = nullptr;           // (rows, pieces) where pieces > 1
+  const float *dy = nullptr;        // log-prob: (rows), else (1) or null for 1
+  float dy_scale = 1.f;
+  void *dx = nullptr;               // (rows, V)
+  int64_t piece = 0;                // set by the launcher
+};
+}  // namespace sa
+// workgroups the launcher takes for each row
+int sa_token_loss_pieces(int64_t rows, int64_t V);
+int sa_token_loss_fwd(int dtype, const sa::TokenLossDesc *d, hipStream_t s);
+int sa_token_loss_bwd(int dtype, const sa::TokenLossDesc *d, hipStream_t s);
+
+// ---- rotary.hip --------------------------------------------------------------
+// Rotary positions of one or two tensors (queries and keys) of shape
+// (B, S, H, D) with a contiguous last dimension, optionally after the
+// root-mean-square norm of every head with scale w (D,).  `y` (forward) / the
+// input gradient (backward, also `y`) is contiguous (B, S, H, D).  freq: host
+// array of R / 2 turns per position, as fractions of 2^64.  pos: null for
+// 0 .. S - 1, or int32 with strides over (B, S).
+namespace sa {
+constexpr int kRotaryMaxDim = 1024;
+constexpr int kRotaryMaxPairs = 256;
+constexpr int kRotaryMaxBlocks = 2048;  // rows of `partial` at most
+struct RotaryTensor {
+  const void *x = nullptr, *dy = nullptr, *w = nullptr;
+  void *y = nullptr, *dw = nullptr;
+  float *partial = nullptr;   // backward of the norm: kRotaryMaxBlocks x D
+  int64_t x_stride[3] = {0, 0, 0}, dy_stride[3] = {0, 0, 0};
+  int H = 0;
+};
+struct RotaryDesc {
+  int parts = 1;
+  RotaryTensor part[2];
+  const int *pos = nullptr;
+  int64_t pos_stride[2] = {0, 0};
+  int64_t B = 0, S = 0;
+  int D = 0, R = 0, half = 1, norm = 0;
+  float eps = 0.f, amplitude = 1.f;
+  const uint64_t *freq = nullptr;
+};
+}  // namespace sa
+int sa_rotary_fwd(int dtype, const sa::RotaryDesc *d, hipStream_t s);
+int sa_rotary_bwd(int dtype, const sa::RotaryDesc *d, hipStream_t s);
+
 // ---- index.hip -----------------------------------------------------------------------------------------------
 // out[o, j, i] = x[o, idx[j], i]   (x: outer x n_in x inner)
 int sa_index_select(int dtype, const void *x, const int *idx, void *out,

@@ -785,6 +785,36 @@ class LayerNorm(Layer):
         return autograd.layer_norm(x, self.scale, self.bias, self.eps)
 
 
+class RotaryQK(Layer):
+    """Rotary positions of queries and keys (batch, sequence, heads,
+    head_dim), with the learned root-mean-square norm of their heads in the
+    same pass when ``norm`` is set; one kernel per direction.
+    ``forward(q, k, positions=None)`` returns both.  The options are those of
+    ``singa_wrap.RotaryHandle``."""
+
+    def __init__(self, rotary_dim=None, base=10000.0, layout="half",
+                 scaling=None, norm=False, eps=1e-6):
+        super().__init__()
+        _keep(self, locals(), 'rotary_dim', 'base', 'layout', 'scaling',
+              'norm', 'eps')
+
+    def initialize(self, q, k, positions=None):
+        d = q.shape[-1]
+        self.handle = singa.RotaryHandle(d, self.rotary_dim, self.base,
+                                         self.layout, self.scaling)
+        if self.norm:
+            self._new_param('q_scale', (d,), q, _constant(1.0), q.dtype)
+            self._new_param('k_scale', (d,), q, _constant(1.0), q.dtype)
+
+    def forward(self, q, k, positions=None):
+        scales = ()
+        if self.norm:
+            scales = (self.q_scale, self.k_scale)
+            self.device_check(q, *scales)
+        return autograd.rotary_qk(self.handle, q, k, positions, *scales,
+                                  eps=self.eps)
+
+
 # ---------------------------------------------------------------------------
 # layers that only forward to an autograd function
 # ---------------------------------------------------------------------------
@@ -823,6 +853,9 @@ Flatten = _functional('Flatten', 'flatten', axis=1)
 Cat = _functional('Cat', 'cat', "forward(list of tensors)", axis=0)
 SoftMaxCrossEntropy = _functional('SoftMaxCrossEntropy',
                                   'softmax_cross_entropy')
+PreferenceLoss = _functional('PreferenceLoss', 'preference_loss',
+                             "forward(x, t, reference)", beta=0.1,
+                             smoothing=0.0)
 MeanSquareError = _functional('MeanSquareError', 'mse_loss')
 CrossEntropy = _functional('CrossEntropy', 'cross_entropy')
 BinaryCrossEntropy = _functional('BinaryCrossEntropy', 'binary_cross_entropy')

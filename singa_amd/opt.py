@@ -447,6 +447,115 @@ class Adam(_Adaptive):
         return self.beta_1_value.data, self.beta_2_value.data
 
 
+class AdamW(Optimizer):
+    """Adam with decoupled weight decay and bias correction (t counts from 1):
+
+        m <- b1 * m + (1 - b1) * g ;  v <- b2 * v + (1 - b2) * g^2
+        p <- p - lr * weight_decay * p
+               - lr * (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+
+    all parameters of a type in one launch for every 48 of them.  16-bit
+    parameters step a float32 master copy (``master_weights``) and are rounded
+    from it; the moments are float32, or 8 bits with ``state_bits=8``: a fifth
+    of their memory (2 bytes and two float scales for each 256 elements instead of
+    8 bytes).  The 8-bit moments m and r = sqrt(v) are e4m3 numbers relative to
+    the largest of their 256; they are rounded stochastically with random
+    bits that depend on ``seed``, the step and the place alone, so a run can
+    be repeated, and resumed from ``get_states()``, exactly.
+
+    ``get_states`` / ``set_states`` carry tables named after the moments:
+    ``m``, ``v`` or ``m``, ``r`` (int32 words of four codes), ``m_scale``,
+    ``r_scale``, and ``masters``."""
+
+    def __init__(self, lr=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-8,
+                 weight_decay=0.01, state_bits=32, master_weights=True,
+                 seed=0):
+        super(AdamW, self).__init__(lr)
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits is 8 or 32, got %r" % (state_bits,))
+        self.state_bits, self.seed = state_bits, int(seed)
+        self.master_weights = master_weights
+        self._hyper("weight_decay", weight_decay, "decay_value",
+                    non_negative=True)
+        self._hyper("beta_1", beta_1, "beta_1_value")
+        self._hyper("beta_2", beta_2, "beta_2_value")
+        self._hyper("epsilon", epsilon, "epsilon_value")
+        self.state_names = ('m', 'v') if state_bits == 32 else \
+            ('m', 'r', 'm_scale', 'r_scale')
+        for name in self.state_names:
+            setattr(self, name, dict())
+        self.masters = dict()
+
+    def _table(self, name, keys, params):
+        """The state tensors ``name`` of these parameters, as core tensors."""
+        table = getattr(self, name)
+        out = []
+        for key, p in zip(keys, params):
+            shape, dtype = p.shape, tensor.float32
+            if self.state_bits == 8:
+                blocks = -(-p.size() // singa.ADAMW_BLOCK)
+                shape = (blocks,) if name.endswith("_scale") else \
+                    (blocks * singa.ADAMW_BLOCK // 4,)
+                dtype = tensor.float32 if name.endswith("_scale") \
+                    else tensor.int32
+            t = table.get(key)
+            if t is not None and (tuple(t.shape) != tuple(shape) or
+                                  t.dtype != dtype):
+                raise ValueError(
+                    "state %s of %s is %s, the parameter needs %s" %
+                    (name, key, tuple(t.shape), tuple(shape)))
+            if t is None:
+                def make(shape=shape, dtype=dtype, dev=p.device):
+                    t = Tensor(shape, dev, dtype)
+                    t.set_value(0)
+                    return t
+                t = table[key] = _eagerly(p.device, make)
+            elif t.device.id() != p.device.id():
+                # adopted from a checkpoint read on the host
+                _eagerly(p.device, lambda t=t, p=p: t.to_device(p.device))
+            out.append(t.data)
+        return out
+
+    def _update(self, items, scale):
+        params = [p for _, p, _ in items]
+        lead = params[0]
+        self.device_check(lead, self.step_counter, *self._values())
+        keys = [self._state_key(n, p) for n, p, _ in items]
+        masters = None
+        if self.master_weights and lead.dtype != tensor.float32:
+            masters = [self._slot(self.masters, k, p, tensor.float32,
+                                  copy=True).data
+                       for k, p in zip(keys, params)]
+        states = [self._table(n, keys, params) for n in self.state_names]
+        states += [None] * (4 - len(states))
+        hypers = (self.lr_value.data, self.decay_value.data,
+                  self.epsilon_value.data, self.beta_1_value.data,
+                  self.beta_2_value.data, self.step_counter.data)
+        singa.AdamWUpdateMulti([p.data for p in params],
+                               [g.data for _, _, g in items], masters, *states,
+                               hypers, self.state_bits, scale, self.seed)
+
+    sync_masters = SGD.sync_masters
+    forget_masters = SGD.forget_masters
+
+    def get_states(self):
+        states = super(AdamW, self).get_states()
+        for n in self.state_names:
+            states[n] = getattr(self, n)
+        if self.masters:
+            states['masters'] = self.masters
+        return states
+
+    def set_states(self, states):
+        other = {'v', 'r', 'm_scale', 'r_scale'} - set(self.state_names)
+        if any(states.get(n) for n in other):
+            raise ValueError("these states are not of %d bits" %
+                             self.state_bits)
+        super(AdamW, self).set_states(states)
+        for n in self.state_names + ('masters',):
+            self._restore(getattr(self, n), states.get(n, {}))
+
+
 # ---------------------------------------------------------------------------
 # data-parallel wrapper
 # ---------------------------------------------------------------------------

@@ -17,6 +17,9 @@ from .core.tensor_core import (Tensor, VecTensor, Product, SizeOf, __add__,
                                __gt__, __ge__, __eq__, _submit)
 from .core.nn_ops import *  # noqa: F401,F403
 from .core.rnn_ops import *  # noqa: F401,F403
+from .core.lm_ops import (RotaryHandle, RotaryForward, RotaryBackward,
+                          TokenLoss, LOSS_LOG_PROB, LOSS_PREFERENCE,
+                          LOSS_POLICY, AdamWUpdateMulti, ADAMW_BLOCK)
 from .parallel.communicator import Communicator, NcclIdHolder
 
 CudaGPU = HipGPU
