@@ -119,34 +119,41 @@ class RotaryHandle(object):
         # turns for each position as fractions of 2^64 (base >= 1: below 2^62)
         self._turns = np.array(
             [round(math.ldexp(v / (2 * math.pi), 64)) for v in f], np.uint64)
+        self.turns_address = self._turns.ctypes.data
+        self.half = layout == "half"
+
+
+def _described(t):
+    return "%s %s" % (tuple(t._shape), dtypes.name(t._dtype))
 
 
 def _check_rotary(handle, xs, scales, positions):
     _refuse(not 1 <= len(xs) <= 2, "rotary takes one or two tensors")
-    lead = xs[0]
+    lead, D = xs[0], handle.head_dim
+    B, S = lead._shape[:2] if lead.nDim() == 4 else (0, 0)
     for x in xs:
         _float_operand("a rotary operand", x)
-        _refuse(x.nDim() != 4 or x._shape[-1] != handle.head_dim,
-                "a rotary operand is (batch, sequence, heads, %d), got %s",
-                handle.head_dim, tuple(x._shape))
-        _refuse(x._shape[:2] != lead._shape[:2] or x._dtype != lead._dtype,
-                "queries and keys share batch, sequence and type: %s %s, "
-                "%s %s", tuple(lead._shape), dtypes.name(lead._dtype),
-                tuple(x._shape), dtypes.name(x._dtype))
-    B, S = lead._shape[:2]
+        shape = x._shape
+        if len(shape) != 4 or shape[3] != D:
+            raise ValueError("a rotary operand is (batch, sequence, heads, "
+                             "%d), got %s" % (D, tuple(shape)))
+        if shape[0] != B or shape[1] != S or x._dtype != lead._dtype:
+            raise ValueError("queries and keys share batch, sequence and "
+                             "type: %s, %s" % (_described(lead),
+                                               _described(x)))
+        _refuse(shape[2] > 65536, "more than 65536 heads")
     _refuse(B * S > 0x7fffffff, "more than 2^31 - 1 tokens in one call")
-    _refuse(any(x._shape[2] > 65536 for x in xs), "more than 65536 heads")
     if scales:
         _refuse(len(scales) != len(xs), "one scale for each tensor")
         for w in scales:
-            _refuse(w._shape != [handle.head_dim] or w._dtype != lead._dtype,
-                    "a scale is (%d,) of the operands' type, got %s %s",
-                    handle.head_dim, tuple(w._shape), dtypes.name(w._dtype))
+            if w._shape != [D] or w._dtype != lead._dtype:
+                raise ValueError("a scale is (%d,) of the operands' type, got "
+                                 "%s" % (D, _described(w)))
     if positions is not None:
         _int_operand("positions", positions)
-        _refuse(positions._shape not in ([S], [B, S]),
-                "positions are (%d,) or (%d, %d), got %s", S, B, S,
-                tuple(positions._shape))
+        if positions._shape != [S] and positions._shape != [B, S]:
+            raise ValueError("positions are (%d,) or (%d, %d), got %s" %
+                             (S, B, S, tuple(positions._shape)))
 
 
 def _rotary(name, handle, xs, scales, positions, eps, dys):
@@ -155,35 +162,29 @@ def _rotary(name, handle, xs, scales, positions, eps, dys):
     _check_rotary(handle, xs, scales, positions)
     eps = float(eps)
     _refuse(not eps >= 0.0, "eps is a number from 0, got %r", eps)
-    dev, n = xs[0]._dev, len(xs)
-    back = dys is not None
+    dev, back = xs[0]._dev, dys is not None
     if back:
         for x, g in zip(xs, dys):
-            _refuse(g._shape != x._shape or g._dtype != x._dtype,
-                    "a gradient of %s %s for an output of %s %s",
-                    tuple(g._shape), dtypes.name(g._dtype), tuple(x._shape),
-                    dtypes.name(x._dtype))
+            if g._shape != x._shape or g._dtype != x._dtype:
+                raise ValueError("a gradient of %s for an output of %s" %
+                                 (_described(g), _described(x)))
         dys = [_rows_contiguous(g) for g in dys]
     # the backward pass of a rotation alone does not need its input
     inputs = [] if back and not scales else [_rows_contiguous(x) for x in xs]
     grads = dys if back else []
     scales = [Contiguous(w) for w in scales]
     ys = [Tensor(x._shape, dev, x._dtype) for x in xs]
-    dws = [Tensor([handle.head_dim], dev, w._dtype) for w in scales] \
-        if back else []
+    dws = [Tensor(w._shape, dev, w._dtype) for w in scales] if back else []
     at = [positions] if positions is not None else []
     reads = inputs + grads + scales + at
-    counts = (len(inputs), len(grads), len(scales), len(at), len(ys),
-              len(dws))
+    ends = []
+    for group in (inputs, grads, scales, at, ys):
+        ends.append((ends[-1] if ends else 0) + len(group))
 
     def body(*ts):
-        parts, k = [], 0
-        for c in counts:
-            parts.append([t.view() for t in ts[k:k + c]])
-            k += c
-        x, g, w, p, y, dw = parts
-        ts[0]._dev.math.rotary(handle, x, g, w, p[0] if p else None, y, dw,
-                               eps)
+        i, g, w, p, y = ends
+        dev.math.rotary(handle, ts[:i], ts[i:g], ts[g:w],
+                        ts[w] if p > w else None, ts[p:y], ts[y:], eps)
 
     _one_device(name, dev, reads)
     _submit(dev, name, body, reads, ys + dws)
@@ -255,29 +256,27 @@ class TokenLoss(object):
         float32."""
         dev, rows, f32 = self.x._dev, self.rows, dtypes.kFloat32
         logp = self.mode == LOSS_LOG_PROB
-        value = Tensor(self.label._shape, dev, f32)
+        # the result of each row is the log-probabilities' output, else kept
         # of each row the largest logit and the log of the sum relative to it,
         # then the derivative (policy), then what rows' derivatives are
         # multiplied by (policy: one number, preference: one for each pair)
-        n = {LOSS_LOG_PROB: 2 * rows, LOSS_PREFERENCE: 2 * rows + self.pairs,
-             LOSS_POLICY: 3 * rows + 1}[self.mode]
+        n = {LOSS_LOG_PROB: 2 * rows, LOSS_PREFERENCE: 3 * rows + self.pairs,
+             LOSS_POLICY: 4 * rows + 1}[self.mode]
         self.saved = Tensor([n], dev, f32)
-        loss = value if logp else Tensor([1], dev, f32)
+        loss = Tensor(self.label._shape if logp else [1], dev, f32)
         given = [t for t in self.extra if t is not None]
         here = [t is not None for t in self.extra]
         ins = [self.x, self.label] + given
         spec = (self.mode, rows, self.V, self.pairs, self.seq, self.consts)
 
         def body(*ts):
-            rest = iter(t.flat() for t in ts[2:2 + len(given)])
+            flat = [t._storage() for t in ts]
+            rest = iter(flat[2:])
             extra = [next(rest) if h else None for h in here]
-            val, saved = ts[2 + len(given)], ts[3 + len(given)]
-            ts[0]._dev.math.token_loss_fwd(
-                spec, ts[0].flat(), ts[1].flat(), extra, val.flat(),
-                saved.flat(), None if logp else ts[-1].flat())
+            dev.math.token_loss_fwd(spec, flat[0], flat[1], extra, flat[-2],
+                                    flat[-1])
 
-        outs = [value, self.saved] + ([] if logp else [loss])
-        _submit(dev, "TokenLossForward", body, ins, outs)
+        _submit(dev, "TokenLossForward", body, ins, [self.saved, loss])
         return loss
 
     def backward(self, dy):
@@ -298,11 +297,10 @@ class TokenLoss(object):
         spec = (self.mode, self.rows, self.V, self.pairs, self.seq)
 
         def body(*ts):
-            w = ts[3].flat() if weight else None
-            g = ts[3 + len(weight)].flat() if dys else None
-            ts[0]._dev.math.token_loss_bwd(spec, ts[0].flat(), ts[1].flat(),
-                                           ts[2].flat(), w, g, scale,
-                                           ts[-1].flat())
+            flat = [t._storage() for t in ts]
+            dev.math.token_loss_bwd(spec, *flat[:3],
+                                    flat[3] if weight else None,
+                                    flat[-2] if dys else None, scale, flat[-1])
 
         reads = [self.x, self.label, self.saved] + weight + dys
         _one_device("TokenLossBackward", dev, reads)
@@ -316,40 +314,45 @@ class TokenLoss(object):
 ADAMW_BLOCK = 256       # values that share the scale of an 8-bit state
 
 
-def AdamWUpdateMulti(params, grads, masters, state1, state2, scales1, scales2,
-                     hypers, state_bits=32, scale=1.0, seed=0):
-    """One AdamW step for a list of parameters of one type (one graph node,
-    one launch for every 48 tensors).  masters: float32 copies of 16-bit
-    parameters, or None.  state_bits 32: state1 / state2 are the float32
-    moments; 8: int32 words of four e4m3 codes of the first moment and of the
-    root of the second, in whole blocks of 256 values, with float32 scales1 /
-    scales2 for each block.  hypers = (lr, weight_decay, epsilon, beta_1,
-    beta_2, step): one-element float32 tensors."""
-    n, dev = len(params), params[0]._dev
-    grads = [g if g._dtype == p._dtype else g.AsType(p._dtype)
-             for p, g in zip(params, grads)]
-    lists = [list(params), [Contiguous(g) for g in grads],
-             list(masters or ()), list(state1), list(state2),
-             list(scales1 or ()), list(scales2 or ())]
-    for p in params:
-        _refuse(not p.is_contiguous(), "AdamW steps contiguous parameters")
+def AdamWUpdateMulti(params, grads, states, mixed, hypers, state_bits=32,
+                     scale=1.0, seed=0):
+    """One AdamW step for a list of contiguous parameters of one type (one
+    graph node, one launch for every 48 tensors).  states: for each parameter
+    its tensors (m, v) -- float32, of the parameter's shape -- or, with
+    state_bits 8, (m, r, m_scale, r_scale): int32 words of four e4m3 codes of
+    the first moment and of the root of the second, in whole blocks of 256
+    values, and a float32 scale for each block; behind them, when ``mixed``,
+    the float32 master copy of a 16-bit parameter.  hypers = (lr,
+    weight_decay, epsilon, beta_1, beta_2, step): one-element float32
+    tensors."""
+    dev, n = params[0]._dev, len(params)
+    dtype = params[0]._dtype
+    columns = list(zip(*states))
+    aligned = []
+    for p, g in zip(params, grads):
+        if g._dtype != dtype:
+            g = g.AsType(dtype)
+        if g._stride != p._stride:
+            g = Contiguous(g)
+        aligned.append(g)
     scale, seed, state_bits = float(scale), int(seed), int(state_bits)
-    written = [i for i in (0, 2, 3, 4, 5, 6) if lists[i]]
-    reads = [t for ts in lists for t in ts] + list(hypers)
-    sizes = [len(ts) for ts in lists]
+    sizes = [p.Size() for p in params]
+    reads = [*params, *aligned]
+    for c in columns:
+        reads += c
+    reads += hypers
+    _one_device("AdamWUpdateMulti", dev, reads)
+    width = 2 + len(columns)
 
     def body(*ts):
-        # the outputs stand behind the inputs: for a recorded step they are
-        # the same blocks
-        parts, k = [], 0
-        for c in sizes:
-            parts.append([t.flat() for t in ts[k:k + c]])
-            k += c
-        hyp = [t.flat() for t in ts[k:k + len(hypers)]]
-        ts[0]._dev.math.adamw_update_multi(
-            [t.Size() for t in ts[:n]], *parts, *hyp, state_bits, scale, seed)
+        # the outputs stand behind the inputs: they are the same blocks
+        flat = [t._storage() for t in ts[:width * n + 6]]
+        cols = [flat[i * n:(i + 1) * n] for i in range(width)]
+        dev.math.adamw_update_multi(sizes, cols, bool(mixed), flat[width * n:],
+                                    state_bits, scale, seed)
 
-    _one_device("AdamWUpdateMulti", dev, reads)
-    _submit(dev, "AdamWUpdateMulti", body, reads,
-            [t for i in written for t in lists[i]])
+    writes = list(params)
+    for c in columns:
+        writes += c
+    _submit(dev, "AdamWUpdateMulti", body, reads, writes)
     return params

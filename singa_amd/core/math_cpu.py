@@ -475,12 +475,15 @@ class CpuMath(object):
             p.copy_(pv - lr * upd)
 
     # ---- AdamW (same contract as the HIP backend) --------------------------------
-    def adamw_update_multi(self, sizes, ps, gs, masters, s1, s2, sc1, sc2, lr,
-                           wd, eps, b1, b2, step, state_bits, scale, seed):
+    def adamw_update_multi(self, sizes, columns, mixed, hypers, state_bits,
+                           scale, seed):
+        ps, gs, s1, s2 = columns[:4]
+        sc1, sc2 = columns[4:6] if state_bits == 8 else (None, None)
+        masters = columns[-1] if mixed else None
         one = np.float32(1.0)
         lr, wd, eps, b1, b2 = (np.float32(t.reshape(-1)[0].item())
-                               for t in (lr, wd, eps, b1, b2))
-        step = int(step.reshape(-1)[0].item())
+                               for t in hypers[:5])
+        step = int(hypers[5].reshape(-1)[0].item())
         # 1 - b^t from 1 - b as float32 holds it
         c1, c2 = (float(-np.expm1((step + 1) * np.log1p(-np.float64(one - b))))
                   for b in (b1, b2))
@@ -512,9 +515,10 @@ class CpuMath(object):
 
     # ---- rotary positions ---------------------------------------------------------
     def rotary(self, handle, xs, dys, ws, pos, ys, dws, eps):
-        B, S = ys[0].shape[:2]
-        R, half = handle.rotary_dim, handle.layout == "half"
-        at = torch.arange(S) if pos is None else pos
+        S, R, half = ys[0]._shape[1], handle.rotary_dim, handle.half
+        xs, dys, ws, ys, dws = ([t.view() for t in ts]
+                                for ts in (xs, dys, ws, ys, dws))
+        at = torch.arange(S) if pos is None else pos.view()
         angle = at.double().unsqueeze(-1) * torch.from_numpy(handle.frequencies)
         cos = (handle.amplitude * torch.cos(angle)).unsqueeze(-2)
         sin = (handle.amplitude * torch.sin(angle)).unsqueeze(-2)
@@ -553,7 +557,7 @@ class CpuMath(object):
             used = used & (weight[:rows] != 0)
         return used, torch.where(used, label, 0).long().unsqueeze(-1)
 
-    def token_loss_fwd(self, spec, x, label, extra, value, saved, loss):
+    def token_loss_fwd(self, spec, x, label, extra, saved, loss):
         mode, rows, V, pairs, seq, consts = spec
         beta, smooth, lo, hi, kl = consts
         ref, old, adv, weight = [None if t is None else t[:rows].double()
@@ -567,12 +571,12 @@ class CpuMath(object):
         for i, kept in enumerate((top, norm)):
             saved[i * rows:(i + 1) * rows].copy_(
                 torch.where(used, kept.squeeze(-1), zero))
-        saved = saved[2 * rows:]
+        value, saved = saved[2 * rows:3 * rows], saved[3 * rows:]
         if mode == 0:
-            value[:rows].copy_(torch.where(used, lp, zero))
+            loss[:rows].copy_(torch.where(used, lp, zero))
         elif mode == 1:
             each = torch.where(used, lp - ref, zero)
-            value[:rows].copy_(each)
+            value.copy_(each)
             side = each.view(2, pairs, seq).sum(-1)
             z = beta * (side[0] - side[1])
             loss.copy_(((1 - smooth) * F.softplus(-z) +
@@ -593,7 +597,7 @@ class CpuMath(object):
                 each = each + kl * (torch.expm1(d) - d)
                 c = c - kl * torch.expm1(d)
             each = torch.where(used, w * each, zero)
-            value[:rows].copy_(each)
+            value.copy_(each)
             total = w.sum()
             total = total if float(total) > 0 else torch.ones_like(total)
             loss.copy_(each.sum() / total)
@@ -604,7 +608,7 @@ class CpuMath(object):
         mode, rows, V, pairs, seq = spec
         used, at = self._token_rows(mode, x, label, rows, V, weight)
         top, norm = saved[:2 * rows].double().view(2, rows, 1)
-        saved = saved[2 * rows:]
+        saved = saved[3 * rows:]
         if mode == 0:
             c = dy[:rows].double()
         else:

@@ -127,6 +127,8 @@ _CONV_SIDE_ZERO = os.environ.get("SINGA_CONV_SIDE_ZERO", "1") != "0"
 _CONV3X3_GEMM_MIN_HW = int(os.environ.get("SINGA_CONV3X3_GEMM_MIN_HW", "2000"))
 
 _NOTHING = contextlib.nullcontext()
+_NO_STRIDES = (0, 0, 0)
+_CODE_OF = {dtypes.from_torch(t): c for t, c in _CODE.items()}
 
 
 def _raw_stream(index):
@@ -1766,78 +1768,80 @@ class HipMath(object):
             [p.numel() for p in ps], ptr[0], ptr[1], ptr[2], ptr[3], ptr[4],
             ptr[5], float(scale), self._s())
 
-    def adamw_update_multi(self, sizes, ps, gs, masters, s1, s2, sc1, sc2, lr,
-                           wd, eps, b1, b2, step, state_bits, scale, seed):
-        """One AdamW step on a list of flat parameters of one type, one launch
-        per 48 tensors (see lm_ops.AdamWUpdateMulti)."""
-        def ptrs(ts):
-            return [t.data_ptr() for t in ts]
-
+    def adamw_update_multi(self, sizes, columns, mixed, hypers, state_bits,
+                           scale, seed):
+        """One AdamW step on flat tensors, one launch per 48 parameters.
+        columns: lists of the parameters, gradients, states (in the order of
+        lm_ops.AdamWUpdateMulti) and, when ``mixed``, float masters."""
+        at = [[t.data_ptr() for t in c] for c in columns]
+        master = at.pop() if mixed else []
+        if state_bits == 32:
+            at += [[], []]
         with self._current():
             self.k.adamw_update_multi(
-                _code(ps[0]), state_bits, ptrs(ps), ptrs(gs), ptrs(masters),
-                ptrs(s1), ptrs(s2), ptrs(sc1), ptrs(sc2), sizes, lr.data_ptr(),
-                wd.data_ptr(), eps.data_ptr(), b1.data_ptr(), b2.data_ptr(),
-                step.data_ptr(), scale, seed & 0xffffffffffffffff, self._s())
+                _code(columns[0][0]), state_bits, at[0], at[1], master,
+                *at[2:], sizes, *[t.data_ptr() for t in hypers], scale,
+                seed & 0xffffffffffffffff, self._s())
 
     # ---- rotary positions ---------------------------------------------------------
     def rotary(self, handle, xs, dys, ws, pos, ys, dws, eps):
-        """Forward without ``dys``, else backward: xs (empty for a rotation
-        alone) and dys (B, S, H, D) views with a contiguous last dimension, ys
-        and dws contiguous outputs (see lm_ops.RotaryForward)."""
+        """Forward without ``dys``, else backward, on core tensors: xs (empty
+        for a rotation alone) and dys (B, S, H, D) with a contiguous last
+        dimension, ys and dws contiguous outputs (lm_ops.RotaryForward)."""
         back = bool(dys)
-        B, S, _, D = ys[0].shape
-        none = (0, 0, 0)
-        keep, parts = [], []
+        B, S, _, D = ys[0]._shape
+        keep, parts = None, []
+        if dws:
+            each = self.k.ROTARY_MAX_BLOCKS * D
+            keep = self._tmp(each * len(dws))
         for i, y in enumerate(ys):
             x, g = xs[i] if xs else None, dys[i] if back else None
-            part = 0
-            if dws:
-                t = self._tmp(self.k.ROTARY_MAX_BLOCKS * D)
-                keep.append(t)
-                part = t.data_ptr()
             parts.append((
-                x.data_ptr() if xs else 0, g.data_ptr() if back else 0,
-                ws[i].data_ptr() if ws else 0, y.data_ptr(),
-                dws[i].data_ptr() if dws else 0, part, y.shape[2],
-                x.stride()[:3] if xs else none,
-                g.stride()[:3] if back else none))
+                x._storage().data_ptr() if xs else 0,
+                g._storage().data_ptr() if back else 0,
+                ws[i]._storage().data_ptr() if ws else 0,
+                y._storage().data_ptr(),
+                dws[i]._storage().data_ptr() if dws else 0,
+                keep.data_ptr() + 4 * each * i if dws else 0, y._shape[2],
+                x._stride[:3] if xs else _NO_STRIDES,
+                g._stride[:3] if back else _NO_STRIDES))
         at = (0, 0) if pos is None else \
-            (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
+            (0, pos._stride[0]) if len(pos._shape) == 1 else pos._stride
         with self._current():
-            self.k.rotary(_code(ys[0]), back, parts,
-                          0 if pos is None else pos.data_ptr(), at, B, S, D,
-                          handle.rotary_dim, handle.layout == "half",
-                          bool(ws), eps, handle.amplitude,
-                          handle._turns.ctypes.data, self._s())
+            self.k.rotary(_CODE_OF[ys[0]._dtype], back, parts,
+                          0 if pos is None else pos._storage().data_ptr(), at,
+                          B, S, D, handle.rotary_dim, handle.half, bool(ws),
+                          eps, handle.amplitude, handle.turns_address,
+                          self._s())
 
     # ---- losses over token log-probabilities ------------------------------------------
-    def token_loss_fwd(self, spec, x, label, extra, value, saved, loss):
-        """lm_ops.TokenLoss.forward on flat operands."""
+    def token_loss_fwd(self, spec, x, label, extra, saved, out):
+        """lm_ops.TokenLoss.forward on flat operands.  saved: for each row the
+        largest logit, the log of the sum, the row's result (unless ``out`` is
+        that), for the policy loss its derivative; then the totals."""
         mode, rows, V, pairs, seq, consts = spec
-        saved_at = saved.data_ptr()
+        at, row = saved.data_ptr(), 4 * rows
         pieces = self.k.token_loss_pieces(rows, V)
         part = self._tmp(2 * rows * pieces) if pieces > 1 else None
         sums = self._tmp(2 * pairs, torch.float64) if pairs else None
-        at = (saved_at, saved_at + 4 * rows, value.data_ptr(),
-              saved_at + 8 * rows, saved_at + (12 if mode == 2 else 8) * rows,
-              sums.data_ptr() if pairs else 0,
-              part.data_ptr() if pieces > 1 else 0)
+        where = (at, at + row, at + 2 * row if mode else out.data_ptr(),
+                 at + 3 * row, at + (4 if mode == 2 else 3) * row,
+                 sums.data_ptr() if pairs else 0,
+                 part.data_ptr() if pieces > 1 else 0)
         with self._current():
             self.k.token_loss_fwd(
                 _code(x), mode, x.data_ptr(), label.data_ptr(), rows, V, pairs,
                 seq, *[0 if t is None else t.data_ptr() for t in extra],
-                consts, at, 0 if loss is None else loss.data_ptr(), self._s())
+                consts, where, out.data_ptr(), self._s())
 
     def token_loss_bwd(self, spec, x, label, saved, weight, dy, dy_scale, dx):
         mode, rows, V, pairs, seq = spec
-        at = saved.data_ptr()
+        at, row = saved.data_ptr(), 4 * rows
         with self._current():
             self.k.token_loss_bwd(
                 _code(x), mode, x.data_ptr(), label.data_ptr(), rows, V, pairs,
-                seq, 0 if weight is None else weight.data_ptr(), at,
-                at + 4 * rows, at + 8 * rows,
-                at + (12 if mode == 2 else 8) * rows,
+                seq, 0 if weight is None else weight.data_ptr(), at, at + row,
+                at + 3 * row, at + (4 if mode == 2 else 3) * row,
                 0 if dy is None else dy.data_ptr(), dy_scale, dx.data_ptr(),
                 self._s())
 

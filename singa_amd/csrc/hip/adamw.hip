@@ -40,7 +40,7 @@ constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // values under one scale: four for each lane
 
 struct Consts {
-  float lr, decay, eps, b1, k1, b2, k2, c1, c2, scale;
+  float lr, decay, eps, b1, k1, b2, k2, c1, c2, root_c2, scale;
 };
 
 __device__ __forceinline__ Consts constants(const AdamwHyper &h) {
@@ -56,6 +56,7 @@ __device__ __forceinline__ Consts constants(const AdamwHyper &h) {
   // 1 - b^t without the cancellation of a b near 1
   c.c1 = 1.f / -expm1f(t * log1pf(-c.k1));
   c.c2 = 1.f / -expm1f(t * log1pf(-c.k2));
+  c.root_c2 = sqrtf(c.c2);
   c.scale = h.scale;
   return c;
 }
@@ -67,6 +68,19 @@ __device__ __forceinline__ void advance(const Consts &c, float g, float &p,
   v = c.b2 * v + c.k2 * (g * g);
   p = p - c.decay * p;
   p = p - c.lr * ((m * c.c1) / (sqrtf(v * c.c2) + c.eps));
+}
+
+// The same with r = sqrt(v) in the place of v.  The step takes the root that
+// the state needs anyway, and a reciprocal good to one unit in the last place.
+__device__ __forceinline__ void advance8(const Consts &c, float g, float &p,
+                                         float &m, float &r) {
+  g = g * c.scale;
+  m = c.b1 * m + c.k1 * g;
+  r = sqrtf(c.b2 * (r * r) + c.k2 * (g * g));
+  const float u =
+      (m * c.c1) * __builtin_amdgcn_rcpf(fmaf(r, c.root_c2, c.eps));
+  p = fmaf(-c.decay, p, p);
+  p = fmaf(-c.lr, u, p);
 }
 
 // the tensor that workgroup `chunk` works on
@@ -179,28 +193,58 @@ __device__ __forceinline__ Words philox(uint32_t c0, uint32_t c1, uint32_t c2,
   return {{c0, c1, c2, c3}};
 }
 
-// the largest finite magnitude of the wave's 256 values
-__device__ __forceinline__ float block_top(const float *x) {
-  float top = 0.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float a = fabsf(x[j]);
-    top = fmaxf(top, a < INFINITY ? a : 0.f);
-  }
-  return wave_max(top);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_dpp(float x) {
+  const int other = __builtin_amdgcn_update_dpp(
+      __float_as_int(x), __float_as_int(x), CTRL, ROWS, 0xf, false);
+  return fmaxf(x, __int_as_float(other));
 }
 
-// x times inv, rounded to e4m3 by the 16 bits of noise
+// The largest of a wave's values, in a scalar register: within rows of 16 lanes
+// (neighbours, pairs, half rows, rows), then into the following rows.
+__device__ __forceinline__ float wave_top(float x) {
+  x = max_dpp<0xb1, 0xf>(x);    // quad_perm 1 0 3 2
+  x = max_dpp<0x4e, 0xf>(x);    // quad_perm 2 3 0 1
+  x = max_dpp<0x141, 0xf>(x);   // row_half_mirror
+  x = max_dpp<0x140, 0xf>(x);   // row_mirror
+  x = max_dpp<0x142, 0xa>(x);   // row_bcast15 into rows 1 and 3
+  x = max_dpp<0x143, 0xc>(x);   // row_bcast31 into rows 2 and 3
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// The largest finite magnitude of the wave's 256 values (NaN loses every
+// comparison of fmaxf; infinities are looked for only where there is one).
+__device__ __forceinline__ float block_top(const float *x) {
+  float top = wave_top(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
+                             fmaxf(fabsf(x[2]), fabsf(x[3]))));
+  if (top == INFINITY) {
+    top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = fabsf(x[j]);
+      top = fmaxf(top, a < INFINITY ? a : 0.f);
+    }
+    top = wave_top(top);
+  }
+  // below this the reciprocal of the scale would overflow: zeros
+  return top > 0x1p-110f ? top : 0.f;
+}
+
+// x times inv, rounded to e4m3 by the 16 bits of noise: floor(s / unit + u) of
+// the codes' spacing.  A normal code keeps three bits of the fraction: the
+// noise is added behind them, a carry goes where it should, the rest is cut
+// off.  Below 2^-6 the spacing is 2^-9 throughout.
 template <bool KEEP>
 __device__ __forceinline__ float to_code(float x, float inv, uint32_t noise) {
   const float s = x * inv, size = fabsf(s);
-  // spacing of the codes around s: an eighth of its binade
-  const float unit =
-      __uint_as_float(__float_as_uint(fmaxf(size, 0x1p-6f)) & 0x7f800000u) *
-      0.125f;
-  float q = floorf(size / unit + (float)noise * 0x1p-16f) * unit;
+  const float normal =
+      __uint_as_float((__float_as_uint(size) + (noise << 4)) & 0xfff00000u);
+  const float small =
+      floorf(size * 512.f + (float)noise * 0x1p-16f) * 0x1p-9f;
+  float q = size < 0x1p-6f ? small : normal;
   if (KEEP) q = size > 0.f ? fmaxf(q, 0x1p-9f) : q;
-  q = q > 448.f ? 448.f : q;   // NaN stays
+  q = q > 448.f ? 448.f : q;
+  q = size < INFINITY ? q : NAN;
   return copysignf(q, s);
 }
 
@@ -264,20 +308,13 @@ __global__ void __launch_bounds__(kThreads)
     float m[4], v[4];
     unpack_codes(m, mc[k], msf[k]);
     unpack_codes(v, rc[k], rsf[k]);
+    // behind the end of the tensor gradients and states are zero and stay so
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = v[j] * v[j];
-      advance(c, gf[k][j], pf[k][j], m[j], v[j]);
-      // behind the end of the tensor the states stay zero
-      m[j] = j < n ? m[j] : 0.f;
-      v[j] = j < n ? sqrtf(v[j]) : 0.f;
-    }
+    for (int j = 0; j < 4; ++j)
+      advance8(c, gf[k][j], pf[k][j], m[j], v[j]);
     store_some<P>(p + i, pf[k], n, wide);
     if (MASTER) store_some<T>(p16 + i, pf[k], n, wide);
-    float mt = block_top(m), rt = block_top(v);
-    // below this the reciprocal of a scale would overflow: zeros
-    mt = mt > 0x1p-110f ? mt : 0.f;
-    rt = rt > 0x1p-110f ? rt : 0.f;
+    const float mt = block_top(m), rt = block_top(v);
     const float mi = mt > 0.f ? 448.f * (1.f / mt) : 0.f;
     const float ri = rt > 0.f ? 448.f * (1.f / rt) : 0.f;
     const int64_t group = (base + i) / 4;

@@ -485,55 +485,96 @@ class AdamW(Optimizer):
         for name in self.state_names:
             setattr(self, name, dict())
         self.masters = dict()
+        self._records = {}      # id(parameter) -> see _record
+        # the constants that the value tensors hold: see _refresh
+        self._held = {a: (getattr(self, a), getattr(self, a).init_value,
+                          getattr(self, v)) for a, v, _ in self._scheduled}
 
-    def _table(self, name, keys, params):
-        """The state tensors ``name`` of these parameters, as core tensors."""
+    def _refresh(self):
+        """As every optimizer's, but a constant whose value is there already
+        costs no launch."""
+        for attr, value_attr, cast in self._scheduled:
+            sched, value = getattr(self, attr), getattr(self, value_attr)
+            if type(sched) is Constant:
+                of, number, at = self._held.get(attr, (None, None, None))
+                if of is sched and number == sched.init_value and at is value:
+                    continue
+                self._held[attr] = (sched, sched.init_value, value)
+            value.copy_from(self._evaluate(sched, cast))
+
+    def _state(self, name, key, p):
+        """The state ``name`` of parameter p, created on first use."""
         table = getattr(self, name)
-        out = []
-        for key, p in zip(keys, params):
-            shape, dtype = p.shape, tensor.float32
-            if self.state_bits == 8:
-                blocks = -(-p.size() // singa.ADAMW_BLOCK)
-                shape = (blocks,) if name.endswith("_scale") else \
-                    (blocks * singa.ADAMW_BLOCK // 4,)
-                dtype = tensor.float32 if name.endswith("_scale") \
-                    else tensor.int32
-            t = table.get(key)
-            if t is not None and (tuple(t.shape) != tuple(shape) or
-                                  t.dtype != dtype):
-                raise ValueError(
-                    "state %s of %s is %s, the parameter needs %s" %
-                    (name, key, tuple(t.shape), tuple(shape)))
-            if t is None:
-                def make(shape=shape, dtype=dtype, dev=p.device):
-                    t = Tensor(shape, dev, dtype)
-                    t.set_value(0)
-                    return t
-                t = table[key] = _eagerly(p.device, make)
-            elif t.device.id() != p.device.id():
-                # adopted from a checkpoint read on the host
-                _eagerly(p.device, lambda t=t, p=p: t.to_device(p.device))
-            out.append(t.data)
-        return out
+        shape, dtype = p.shape, tensor.float32
+        if self.state_bits == 8:
+            blocks = -(-p.size() // singa.ADAMW_BLOCK)
+            if name.endswith("_scale"):
+                shape = (blocks,)
+            else:
+                shape = (blocks * singa.ADAMW_BLOCK // 4,)
+                dtype = tensor.int32
+        t = table.get(key)
+        if t is None:
+            def make():
+                made = Tensor(shape, p.device, dtype)
+                made.set_value(0)
+                return made
+            t = table[key] = _eagerly(p.device, make)
+        elif tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+            raise ValueError("state %s of %s is %s, the parameter needs %s" %
+                             (name, key, tuple(t.shape), tuple(shape)))
+        elif t.device.id() != p.device.id():
+            # adopted from a checkpoint read on the host
+            _eagerly(p.device, lambda: t.to_device(p.device))
+        return t
+
+    def _record(self, name, p):
+        """What a step needs of a parameter beside its gradient: (parameter,
+        core tensor, core type, state key, its state tensors in the order of
+        ``_tables``)."""
+        core = p.data
+        if not core.is_contiguous():
+            raise ValueError("AdamW steps contiguous parameters")
+        key = self._state_key(name, p)
+        held = [self._state(n, key, p) for n in self.state_names]
+        if self.master_weights and p.dtype != tensor.float32:
+            held.append(self._slot(self.masters, key, p, tensor.float32,
+                                   copy=True))
+        r = self._records[id(p)] = (p, core, core.data_type(), name, key, held,
+                                    [t.data for t in held])
+        return r
+
+    def _tables(self, mixed):
+        return [getattr(self, n) for n in self.state_names] + \
+            ([self.masters] if mixed else [])
 
     def _update(self, items, scale):
-        params = [p for _, p, _ in items]
-        lead = params[0]
-        self.device_check(lead, self.step_counter, *self._values())
-        keys = [self._state_key(n, p) for n, p, _ in items]
-        masters = None
-        if self.master_weights and lead.dtype != tensor.float32:
-            masters = [self._slot(self.masters, k, p, tensor.float32,
-                                  copy=True).data
-                       for k, p in zip(keys, params)]
-        states = [self._table(n, keys, params) for n in self.state_names]
-        states += [None] * (4 - len(states))
-        hypers = (self.lr_value.data, self.decay_value.data,
-                  self.epsilon_value.data, self.beta_1_value.data,
-                  self.beta_2_value.data, self.step_counter.data)
-        singa.AdamWUpdateMulti([p.data for p in params],
-                               [g.data for _, _, g in items], masters, *states,
-                               hypers, self.state_bits, scale, self.seed)
+        lead = items[0][1]
+        dev = lead.data.device()
+        hypers = [t.data for t in (self.lr_value, self.decay_value,
+                                   self.epsilon_value, self.beta_1_value,
+                                   self.beta_2_value, self.step_counter)]
+        if any(h.device() is not dev for h in hypers):
+            self.device_check(lead, self.step_counter, *self._values())
+        mixed = self.master_weights and lead.dtype != tensor.float32
+        tables = self._tables(mixed)
+        params, grads, states = [], [], []
+        for name, p, g in items:
+            r = self._records.get(id(p))
+            # the record holds while the parameter and its states are the
+            # tensors it was made of, on this device
+            if r is None or r[0] is not p or r[1] is not p.data or \
+                    r[2] != r[1]._dtype or r[3] != name or \
+                    len(r[5]) != len(tables) or \
+                    any([t.get(r[4]) is not h or h.data is not c or
+                         c._dev is not dev
+                         for t, h, c in zip(tables, r[5], r[6])]):
+                r = self._record(name, p)
+            params.append(r[1])
+            grads.append(g.data)
+            states.append(r[6])
+        singa.AdamWUpdateMulti(params, grads, states, mixed, hypers,
+                               self.state_bits, scale, self.seed)
 
     sync_masters = SGD.sync_masters
     forget_masters = SGD.forget_masters
