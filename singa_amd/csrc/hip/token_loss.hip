@@ -71,6 +71,17 @@ __device__ __forceinline__ Running join(const Running &a, const Running &b) {
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <bool STREAM, typename P>
+__device__ __forceinline__ void put(P *at, const P &v) {
+  if constexpr (STREAM && sizeof(P) == 16)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v),
+                                reinterpret_cast<u32x4 *>(at));
+  else
+    *at = v;
+}
+
 // Elements before the first 16-byte boundary of p, at most n
 template <typename T, int VEC>
 __device__ __forceinline__ int64_t lead(const T *p, int64_t n) {
@@ -176,13 +187,16 @@ __device__ void finish_row(const TokenLossDesc &d, int64_t r, bool used,
   }
 }
 
-// WPR waves of a 256-thread workgroup share a row (1: four rows a workgroup);
-// gridDim.y pieces of a row (only with WPR 4) leave their (maximum, sum) in
-// d.part for the join kernel.
+constexpr int threads_of(int waves) { return waves == 1 ? 256 : 64 * waves; }
+
+// WPR waves share a row, a workgroup has one row (WPR 1: four); gridDim.y
+// pieces of a row (not with WPR 1) leave their (maximum, sum) in d.part for
+// the join kernel.
 template <typename T, int VEC, int WPR>
-__global__ void __launch_bounds__(256) token_rows_kernel(TokenLossDesc d) {
+__global__ void __launch_bounds__(threads_of(WPR))
+    token_rows_kernel(TokenLossDesc d) {
   const int wave = threadIdx.x >> 6;
-  const int64_t r = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;
+  const int64_t r = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   const bool used = r < d.rows && takes_part(d, r);
   Running run;
   if (used) {
@@ -193,11 +207,12 @@ __global__ void __launch_bounds__(256) token_rows_kernel(TokenLossDesc d) {
     run = join_wave(run);
   }
   if (WPR > 1) {   // one row for the whole workgroup: `used` is uniform
-    __shared__ float2 all[4];
+    __shared__ float2 all[WPR];
     if ((threadIdx.x & 63) == 0) all[wave] = make_float2(run.m, run.s);
     __syncthreads();
-    auto of = [&](int i) { return Running{all[i].x, all[i].y}; };
-    run = join(join(of(0), of(1)), join(of(2), of(3)));
+    run = Running{all[0].x, all[0].y};
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) run = join(run, Running{all[i].x, all[i].y});
   }
   if ((threadIdx.x & (64 * WPR - 1)) != 0 || r >= d.rows) return;
   if (WPR > 1 && gridDim.y > 1)
@@ -314,10 +329,12 @@ __global__ void __launch_bounds__(1024)
 // are kept apart: added up, a row of large logits would lose the logarithm.
 // Rows are taken from the last to the first, so that the logits the forward
 // pass read last are met while they are still in the last-level cache.
-template <typename T, int VEC, int WPR>
-__global__ void __launch_bounds__(256) token_grad_kernel(TokenLossDesc d) {
-  const int wave = threadIdx.x >> 6;
-  const int64_t q = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;
+// STREAM: the gradient is stored past the caches.
+template <typename T, int VEC, int WPR, bool STREAM>
+__global__ void __launch_bounds__(threads_of(WPR))
+    token_grad_kernel(TokenLossDesc d) {
+  const int64_t q =
+      WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (q >= d.rows) return;
   const int64_t r = d.rows - 1 - q;
   const int tid = threadIdx.x & (64 * WPR - 1), threads = 64 * WPR;
@@ -346,7 +363,7 @@ __global__ void __launch_bounds__(256) token_grad_kernel(TokenLossDesc d) {
     Pack<T, VEC> z;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) z.v[j] = from_f<T>(0.f);
-    for (int64_t i = tid; i < packs; i += threads) o[i] = z;
+    for (int64_t i = tid; i < packs; i += threads) put<STREAM>(o + i, z);
     if (tid < h) dx[tid] = from_f<T>(0.f);
     if (tid < n - rest) dx[rest + tid] = from_f<T>(0.f);
     return;
@@ -367,7 +384,7 @@ __global__ void __launch_bounds__(256) token_grad_kernel(TokenLossDesc d) {
     Pack<T, VEC> out;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) out.v[j] = from_f<T>(g[j]);
-    o[i] = out;
+    put<STREAM>(o + i, out);
   };
   int64_t i = tid;
   for (; i + (kUnroll - 1) * (int64_t)threads < packs;
@@ -393,28 +410,43 @@ int check_desc(const TokenLossDesc &d) {
   return 0;
 }
 
-// a row for each wave up to this many logits: 64 lanes then have no more than
-// four of the unrolled steps
+// A row for each wave up to this many logits: 64 lanes then have no more than
+// four (16 bits: two) of the unrolled steps.
 constexpr int64_t kWaveRow = 4096;
+// A row (or piece) of at least 32 KB, one unrolled step of 512 threads, is
+// taken by eight waves, a shorter one by four: bf16, both directions, 8192 x
+// 50257 356 us with eight and 377 with four, 4096 x 30522 114 and 119, but
+// 16384 x 10007 (20 KB) 166 and 141.
+constexpr int64_t kLongRow = 32 << 10;
+// A gradient of over half the 256 MB last-level cache is stored past it: it
+// would not stay there for whoever reads it next, and throws out the logits
+// (8192 x 50257 bf16: 356 us instead of 388, 4096 x 30522 114 instead of 134).
+constexpr int64_t kStreamBytes = 128 << 20;
 
 template <typename T, int VEC>
 void launch_rows(const TokenLossDesc &d, int pieces, hipStream_t s) {
   if (d.V <= kWaveRow)
     hipLaunchKernelGGL((token_rows_kernel<T, VEC, 1>),
                        dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, s, d);
-  else
+  else if (d.piece * (int64_t)sizeof(T) < kLongRow)
     hipLaunchKernelGGL((token_rows_kernel<T, VEC, 4>),
                        dim3((unsigned)d.rows, pieces), dim3(256), 0, s, d);
+  else
+    hipLaunchKernelGGL((token_rows_kernel<T, VEC, 8>),
+                       dim3((unsigned)d.rows, pieces), dim3(512), 0, s, d);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool STREAM>
 void launch_grad(const TokenLossDesc &d, int pieces, hipStream_t s) {
   if (d.V <= kWaveRow)
-    hipLaunchKernelGGL((token_grad_kernel<T, VEC, 1>),
+    hipLaunchKernelGGL((token_grad_kernel<T, VEC, 1, STREAM>),
                        dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, s, d);
-  else
-    hipLaunchKernelGGL((token_grad_kernel<T, VEC, 4>),
+  else if (d.piece * (int64_t)sizeof(T) < kLongRow)
+    hipLaunchKernelGGL((token_grad_kernel<T, VEC, 4, STREAM>),
                        dim3((unsigned)d.rows, pieces), dim3(256), 0, s, d);
+  else
+    hipLaunchKernelGGL((token_grad_kernel<T, VEC, 8, STREAM>),
+                       dim3((unsigned)d.rows, pieces), dim3(512), 0, s, d);
 }
 
 // whether every row of a and b has its 16-byte boundaries at the same places
@@ -472,10 +504,12 @@ int sa_token_loss_bwd(int dtype, const TokenLossDesc *desc, hipStream_t s) {
   d.piece = piece_of(d.V, pieces);
   const bool wide = same_phase(d.x, d.dx);
   SA_DISPATCH_FLOAT(dtype, T, {
-    if (wide)
-      launch_grad<T, 16 / (int)sizeof(T)>(d, pieces, s);
+    if (!wide)
+      launch_grad<T, 1, false>(d, pieces, s);
+    else if (d.rows * d.V * (int64_t)sizeof(T) > kStreamBytes)
+      launch_grad<T, 16 / (int)sizeof(T), true>(d, pieces, s);
     else
-      launch_grad<T, 1>(d, pieces, s);
+      launch_grad<T, 16 / (int)sizeof(T), false>(d, pieces, s);
   });
   return 0;
 }
