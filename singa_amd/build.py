@@ -25,9 +25,11 @@ EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 # given wrong results on this chip.  The host pass warns that it does not know
 # the feature.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# sources whose results depend on infinities, NaN or the order of operations
-STRICT_HIP = ("adamw.hip", "rotary.hip", "token_loss.hip")
-STRICT_FLAGS = ["-fno-fast-math", "-ffp-contract=off"]
+# sources whose results depend on infinities and NaN, or (adamw) also on every
+# rounding of the formula
+STRICT_HIP = {"adamw.hip": ["-fno-fast-math", "-ffp-contract=off"],
+              "rotary.hip": ["-fno-fast-math"],
+              "token_loss.hip": ["-fno-fast-math"]}
 # extra hipcc flags for diagnostic builds, e.g. SA_HIPCC_FLAGS=-DSA_CONV_PROF
 EXTRA_HIPCC = os.environ.get("SA_HIPCC_FLAGS", "").split()
 
@@ -105,8 +107,7 @@ def build_hip(force=False, verbose=True):
             jobs.append([hipcc, "--offload-arch=" + ARCH, "-O3", "-std=c++17",
                          "-fPIC", "-ffast-math", "-fno-gpu-rdc",
                          "-Wno-unused-result"] + NO_PACKED_FP32 +
-                        (STRICT_FLAGS if os.path.basename(s) in STRICT_HIP
-                         else []) + EXTRA_HIPCC +
+                        STRICT_HIP.get(os.path.basename(s), []) + EXTRA_HIPCC +
                         ["-c", s, "-o", o])
     bind = os.path.join(CSRC, "bindings", "hip_bind.cc")
     bo = os.path.join(OBJ, "hip_bind.o")

@@ -56,6 +56,7 @@ struct RotaryArgs {
   int S, tokens, D, R;
   int units;          // D / (2 V): what a team of lanes shares
   int lanes;          // of a team: the next power of two of units, at most 64
+  int flat;           // all tensors: batch stride = S times token stride
   int half;           // 1: pairs (i, i + R / 2), 0: pairs (2 i, 2 i + 1)
   float eps, amplitude;
   uint64_t freq[kRotaryMaxPairs];
@@ -63,16 +64,44 @@ struct RotaryArgs {
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T v[V]; };
 
-template <typename T, int V>
-__device__ __forceinline__ void load_unit(float *e, const T *row, int lo,
-                                          int hi) {
-  const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(row + lo);
-  const Vec<T, V> b = *reinterpret_cast<const Vec<T, V> *>(row + hi);
+// the two loads of a unit, as they are in memory
+template <typename T, int V> struct Unit {
+  Vec<T, V> a, b;
+
+  __device__ __forceinline__ void load(const T *row, int lo, int hi, bool ok) {
+    if (ok) {
+      a = *reinterpret_cast<const Vec<T, V> *>(row + lo);
+      b = *reinterpret_cast<const Vec<T, V> *>(row + hi);
+    } else {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    e[j] = to_f<T>(a.v[j]);
-    e[V + j] = to_f<T>(b.v[j]);
+      for (int j = 0; j < V; ++j) a.v[j] = b.v[j] = from_f<T>(0.f);
+    }
   }
+  __device__ __forceinline__ void widen(float *e) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      e[j] = to_f<T>(a.v[j]);
+      e[V + j] = to_f<T>(b.v[j]);
+    }
+  }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  const int other = __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf,
+                                                0xf, false);
+  return x + __int_as_float(other);
+}
+
+// sum over each aligned group of `lanes` lanes (a power of two), in all of them
+__device__ __forceinline__ float group_sum(float x, int lanes) {
+  if (lanes > 1) x = add_dpp<0xb1>(x);    // quad_perm 1 0 3 2
+  if (lanes > 2) x = add_dpp<0x4e>(x);    // quad_perm 2 3 0 1
+  if (lanes > 4) x = add_dpp<0x141>(x);   // row_half_mirror
+  if (lanes > 8) x = add_dpp<0x140>(x);   // row_mirror
+  if (lanes > 16) x += __shfl_xor(x, 16, 64);
+  if (lanes > 32) x += __shfl_xor(x, 32, 64);
+  return x;
 }
 
 template <typename T, int V>
@@ -111,12 +140,14 @@ __device__ __forceinline__ void turn(float *e, const float2 *cs, float sign,
 }
 
 // V: pairs of a unit.  NU: units a lane holds (more than one only where a head
-// has over 64 of them).
+// has over 64 of them).  The loads of a team's next row fly while the present
+// one is computed, and those of a tile's first row while the workgroup computes
+// its table.
 template <typename T, int V, int NU, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, NU == 1 ? 4 : 2)
+    rotary_kernel(RotaryArgs a) {
   __shared__ float2 cs[kTableMax];
-  __shared__ int64_t x_at[kTileMax], g_at[kTileMax];
-  constexpr bool kSums = NORM && BWD;
+  constexpr bool kSums = NORM && BWD, kReadX = !BWD || NORM;
   __shared__ float sums[kSums ? 4 * 128 * V * NU : 1];
   const int which = (int)blockIdx.x >= a.part[0].blocks;
   const RotaryPart &p = a.part[which];
@@ -126,6 +157,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   const int teams = kThreads / a.lanes;
   const int D = a.D, R = a.R, pairs = R >> 1, H = p.H;
   const bool half = a.half != 0;
+  const float inv_D = 1.f / (float)D;
 
   int lo[NU], hi[NU], at[NU];   // element offsets, first pair in the table
   bool mine[NU], turns[NU];
@@ -148,12 +180,42 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
       w[u][j] = 1.f;
       acc[u][j] = 0.f;
     }
-    if (NORM && mine[u]) load_unit<T, V>(w[u], (const T *)p.w, lo[u], hi[u]);
+    if (NORM) {
+      Unit<T, V> raw;
+      raw.load((const T *)p.w, lo[u], hi[u], mine[u]);
+      raw.widen(w[u]);
+    }
   }
 
   for (int tile = block; (int64_t)tile * p.tile < a.tokens; tile += p.blocks) {
     const int first = tile * p.tile;
     const int count = a.tokens - first < p.tile ? a.tokens - first : p.tile;
+    const int rows = count * H;
+    Unit<T, V> x_next[NU], g_next[NU];
+    int t_next = 0, head_next = 0;
+    auto fetch = [&](int row) {
+      const bool ok = row < rows;
+      const int t = !ok ? 0 : p.magic ? (int)__umulhi((unsigned)row, p.magic)
+                                      : row;
+      t_next = t;
+      head_next = ok ? row - t * H : 0;
+      // tokens are one after another in memory, or batches lie apart
+      int64_t b = 0, s = first + t;
+      if (!a.flat) {
+        b = (first + t) / a.S;
+        s -= b * a.S;
+      }
+      const T *xr = (const T *)p.x + b * p.x_sb + s * p.x_ss +
+                    head_next * p.x_sh;
+      const T *gr = (const T *)p.dy + b * p.g_sb + s * p.g_ss +
+                    head_next * p.g_sh;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        if (kReadX) x_next[u].load(xr, lo[u], hi[u], ok && mine[u]);
+        if (BWD) g_next[u].load(gr, lo[u], hi[u], ok && mine[u]);
+      }
+    };
+    fetch(team);
     __syncthreads();   // the previous tile's table has been used
     for (int e = tid; e < count * pairs; e += kThreads) {
       const int t = e / pairs, i = e - t * pairs;
@@ -167,55 +229,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
       sincospif(f, &sn, &c);
       cs[e] = make_float2(c * a.amplitude, sn * a.amplitude);
     }
-    if (tid < count) {
-      const int b = (first + tid) / a.S, s = (first + tid) - b * a.S;
-      x_at[tid] = b * p.x_sb + s * p.x_ss;
-      if (BWD) g_at[tid] = b * p.g_sb + s * p.g_ss;
-    }
     __syncthreads();
-    const int rows = count * H;
     for (int base = 0; base < rows; base += teams) {
-      const int row = base + team;
-      const bool ok = row < rows;
-      const int t = !ok ? 0 : p.magic ? (int)__umulhi((unsigned)row, p.magic)
-                                      : row;
-      const int head = ok ? row - t * H : 0;
-      T *out = (T *)p.y + ((int64_t)(first + t) * H + head) * D;
-      const T *xr = (const T *)p.x + x_at[t] + head * p.x_sh;
+      const bool ok = base + team < rows;
+      const int t = t_next;
+      T *out = (T *)p.y + ((int64_t)(first + t) * H + head_next) * D;
       float e[NU][2 * V], g[NU][2 * V];
-      float sq = 0.f;
-      if (!BWD || NORM) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          if (ok && mine[u]) {
-            load_unit<T, V>(e[u], xr, lo[u], hi[u]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) e[u][j] = 0.f;
-          }
-        }
+      for (int u = 0; u < NU; ++u) {
+        if (kReadX) x_next[u].widen(e[u]);
+        if (BWD) g_next[u].widen(g[u]);
       }
-      if (BWD) {
-        const T *gr = (const T *)p.dy + g_at[t] + head * p.g_sh;
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          if (ok && mine[u]) {
-            load_unit<T, V>(g[u], gr, lo[u], hi[u]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) g[u][j] = 0.f;
-          }
-        }
-      }
+      if (base + teams < rows) fetch(base + teams + team);
       float rstd = 1.f;
       if (NORM) {
+        float sq = 0.f;
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) sq += e[u][j] * e[u][j];
-        for (int off = a.lanes >> 1; off > 0; off >>= 1)
-          sq += __shfl_xor(sq, off, 64);
-        rstd = ok ? 1.f / sqrtf(sq / (float)D + a.eps) : 0.f;
+        // a team without a row: nothing, also where eps is 0
+        rstd = ok ? rsqrtf(group_sum(sq, a.lanes) * inv_D + a.eps) : 0.f;
       }
       if (!BWD) {
 #pragma unroll
@@ -244,11 +278,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
           }
         }
       }
-      if (NORM) {
-        for (int off = a.lanes >> 1; off > 0; off >>= 1)
-          dot += __shfl_xor(dot, off, 64);
-        dot /= (float)D;
-      }
+      if (NORM) dot = group_sum(dot, a.lanes) * inv_D;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         if (!(ok && mine[u])) continue;
@@ -302,8 +332,10 @@ __global__ void __launch_bounds__(1024)
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
   const int d = blockIdx.x * 16 + c;
   float v = 0.f;
-  if (d < D)
+  if (d < D) {
+#pragma unroll 8
     for (int i = r; i < n; i += 64) v += p[(int64_t)i * D + d];
+  }
   s[r][c] = v;
   __syncthreads();
   for (int k = 32; k > 0; k >>= 1) {
@@ -353,12 +385,17 @@ static int rotary_run(int dtype, const RotaryDesc *d, bool bwd, hipStream_t s) {
   a.D = d->D;
   a.R = d->R;
   a.half = d->half;
+  a.flat = 1;
   a.eps = d->eps;
   a.amplitude = d->amplitude;
   for (int i = 0; i < d->R / 2; ++i) a.freq[i] = d->freq[i];
   // pairs of a unit: the widest access that divides the rotated and the passed
   // channels and that every row's address allows
   int V = 16 / size;
+  // the backward pass of the norm holds six values for each of its inputs: with
+  // eight 16-bit pairs a lane it spills (2 x 4096 x 40 heads of 128, bf16: 66 us
+  // instead of 61)
+  if (bwd && d->norm && V > 4) V = 4;
   auto fits = [&](int v) {
     if (d->R % (2 * v) || d->D % (2 * v)) return false;
     // the two halves of the half layout start R / 2 apart: a multiple of v
@@ -393,12 +430,16 @@ static int rotary_run(int dtype, const RotaryDesc *d, bool bwd, hipStream_t s) {
     p.x_sb = t.x_stride[0]; p.x_ss = t.x_stride[1]; p.x_sh = t.x_stride[2];
     p.g_sb = t.dy_stride[0]; p.g_ss = t.dy_stride[1]; p.g_sh = t.dy_stride[2];
     p.H = t.H;
+    if (d->B > 1 && ((t.x && p.x_sb != d->S * p.x_ss) ||
+                     (bwd && p.g_sb != d->S * p.g_ss)))
+      a.flat = 0;
     p.magic = t.H == 1 ? 0 : (unsigned)((0x100000000ull + t.H - 1) / t.H);
-    // about four rows for each team, fewer where that leaves CUs idle
+    // four rows for each team, fewer where that leaves CUs idle (3 x 1021 tokens
+    // of 15 heads: 27 us for both directions, 34 when 1024 tiles are asked for)
     int tile = 4 * teams / t.H;
     tile = tile < 1 ? 1 : tile > kTileMax ? kTileMax : tile;
     while (tile > 1 && tile * pairs > kTableMax) tile >>= 1;
-    while (tile > 1 && a.tokens / tile < 1024) tile >>= 1;
+    while (tile > 1 && a.tokens / tile < 512) tile >>= 1;
     p.tile = tile;
     p.blocks = (a.tokens + tile - 1) / tile;
     if (sums && p.blocks > kRotaryMaxBlocks) p.blocks = kRotaryMaxBlocks;
