@@ -6,7 +6,9 @@ The functions check their arguments on the host (the kernels trust them), and
 submit one named operation each, so that they run eagerly or become a node of
 the recorded step.  The reference has none of them.
 """
+import itertools
 import math
+import operator
 
 import numpy as np
 
@@ -141,8 +143,9 @@ def _check_rotary(handle, xs, scales, positions):
             raise ValueError("queries and keys share batch, sequence and "
                              "type: %s, %s" % (_described(lead),
                                                _described(x)))
-        _refuse(shape[2] > 65536, "more than 65536 heads")
-    _refuse(B * S > 0x7fffffff, "more than 2^31 - 1 tokens in one call")
+        _refuse(not 1 <= shape[2] <= 65536, "1 to 65536 heads, got %d",
+                shape[2])
+    _refuse(B * S > 1 << 30, "more than 2^30 tokens in one call")
     if scales:
         _refuse(len(scales) != len(xs), "one scale for each tensor")
         for w in scales:
@@ -187,7 +190,11 @@ def _rotary(name, handle, xs, scales, positions, eps, dys):
                         ts[w] if p > w else None, ts[p:y], ts[y:], eps)
 
     _one_device(name, dev, reads)
-    _submit(dev, name, body, reads, ys + dws)
+    if xs[0].Size() == 0:
+        for w in dws:      # sums over nothing
+            w.SetFloatValue(0.0)
+    else:
+        _submit(dev, name, body, reads, ys + dws)
     return ys, dws
 
 
@@ -221,7 +228,7 @@ class TokenLoss(object):
                  kl=0.0):
         _float_operand("logits", x)
         _int_operand("a label", label)
-        _refuse(x.nDim() < 1 or x._shape[:-1] != label._shape,
+        _refuse(x.nDim() < 2 or x._shape[:-1] != label._shape,
                 "logits %s need labels %s, got %s", tuple(x._shape),
                 tuple(x._shape[:-1]), tuple(label._shape))
         _refuse(x._shape[-1] < 1, "an empty vocabulary")
@@ -314,45 +321,46 @@ class TokenLoss(object):
 ADAMW_BLOCK = 256       # values that share the scale of an 8-bit state
 
 
+_stored = operator.attrgetter("_block.data")
+_typed = operator.attrgetter("_dtype")
+_held_in = operator.attrgetter("_block")
+_placed = operator.attrgetter("_dev")
+
+
 def AdamWUpdateMulti(params, grads, states, mixed, hypers, state_bits=32,
                      scale=1.0, seed=0):
     """One AdamW step for a list of contiguous parameters of one type (one
-    graph node, one launch for every 48 tensors).  states: for each parameter
-    its tensors (m, v) -- float32, of the parameter's shape -- or, with
+    graph node, one launch for every 48 tensors).  states: lists of the
+    parameters' states, (m, v) -- float32, of the parameter's shape -- or, with
     state_bits 8, (m, r, m_scale, r_scale): int32 words of four e4m3 codes of
     the first moment and of the root of the second, in whole blocks of 256
     values, and a float32 scale for each block; behind them, when ``mixed``,
-    the float32 master copy of a 16-bit parameter.  hypers = (lr,
+    the float32 master copies of 16-bit parameters.  hypers = (lr,
     weight_decay, epsilon, beta_1, beta_2, step): one-element float32
     tensors."""
-    dev, n = params[0]._dev, len(params)
-    dtype = params[0]._dtype
-    columns = list(zip(*states))
-    aligned = []
-    for p, g in zip(params, grads):
-        if g._dtype != dtype:
-            g = g.AsType(dtype)
-        if g._stride != p._stride:
-            g = Contiguous(g)
-        aligned.append(g)
+    dev, n, dtype = params[0]._dev, len(params), params[0]._dtype
+    # the tensors of a launch are stepped side by side
+    _refuse(len(set(map(id, map(_held_in, params)))) != n,
+            "a parameter twice in one step")
+    if {dtype} != set(map(_typed, grads)):
+        grads = [g.AsType(dtype) for g in grads]
+    grads = [g if g._stride == p._stride else Contiguous(g)
+             for p, g in zip(params, grads)]
     scale, seed, state_bits = float(scale), int(seed), int(state_bits)
+    reads = [*params, *grads, *itertools.chain(*states), *hypers]
+    if {dev} != set(map(_placed, reads)):
+        _one_device("AdamWUpdateMulti", dev, reads)
     sizes = [p.Size() for p in params]
-    reads = [*params, *aligned]
-    for c in columns:
-        reads += c
-    reads += hypers
-    _one_device("AdamWUpdateMulti", dev, reads)
-    width = 2 + len(columns)
+    columns = 2 + len(states)
 
     def body(*ts):
         # the outputs stand behind the inputs: they are the same blocks
-        flat = [t._storage() for t in ts[:width * n + 6]]
-        cols = [flat[i * n:(i + 1) * n] for i in range(width)]
-        dev.math.adamw_update_multi(sizes, cols, bool(mixed), flat[width * n:],
-                                    state_bits, scale, seed)
+        flat = list(map(_stored, ts[:columns * n + 6]))
+        flat = [t._storage() if s is None else s for t, s in zip(ts, flat)]
+        dev.math.adamw_update_multi(
+            sizes, [flat[i * n:(i + 1) * n] for i in range(columns)],
+            bool(mixed), flat[columns * n:], state_bits, scale, seed)
 
-    writes = list(params)
-    for c in columns:
-        writes += c
-    _submit(dev, "AdamWUpdateMulti", body, reads, writes)
+    _submit(dev, "AdamWUpdateMulti", body, reads,
+            [*params, *itertools.chain(*states)])
     return params

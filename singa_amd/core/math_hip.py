@@ -1773,7 +1773,7 @@ class HipMath(object):
         """One AdamW step on flat tensors, one launch per 48 parameters.
         columns: lists of the parameters, gradients, states (in the order of
         lm_ops.AdamWUpdateMulti) and, when ``mixed``, float masters."""
-        at = [[t.data_ptr() for t in c] for c in columns]
+        at = [list(map(torch.Tensor.data_ptr, c)) for c in columns]
         master = at.pop() if mixed else []
         if state_bits == 32:
             at += [[], []]

@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? 4 : 2)
     }
   }
 
-  for (int tile = block; (int64_t)tile * p.tile < a.tokens; tile += p.blocks) {
-    const int first = tile * p.tile;
+  for (int64_t tile = block; tile * p.tile < a.tokens; tile += p.blocks) {
+    const int first = (int)(tile * p.tile);
     const int count = a.tokens - first < p.tile ? a.tokens - first : p.tile;
     const int rows = count * H;
     Unit<T, V> x_next[NU], g_next[NU];
@@ -373,7 +373,7 @@ static int rotary_run(int dtype, const RotaryDesc *d, bool bwd, hipStream_t s) {
   if (dtype != kF32 && dtype != kF16 && dtype != kBF16) return -1;
   if (d->D < 2 || d->D > kRotaryMaxDim || (d->D & 1) || d->R < 2 ||
       d->R > d->D || (d->R & 1) || d->R > 2 * kRotaryMaxPairs || d->B < 0 ||
-      d->S < 0 || (int64_t)d->B * d->S > 0x7fffffffll)
+      d->S < 0 || (int64_t)d->B * d->S > 1ll << 30)
     return -2;
   RotaryArgs a;
   a.tokens = (int)(d->B * d->S);

@@ -20,6 +20,8 @@ API parity: reference python/singa/opt.py (DecayScheduler :28-68, Optimizer
 :71-171, SGD :174-333, RMSProp :336-441, AdaGrad :444-533, Adam :536-683,
 DistOpt :686-1094).
 """
+import itertools
+import operator
 from collections import OrderedDict
 
 from . import autograd
@@ -447,6 +449,15 @@ class Adam(_Adaptive):
         return self.beta_1_value.data, self.beta_2_value.data
 
 
+_core = operator.attrgetter("data")
+_device = operator.attrgetter("_dev")
+
+
+def _same(a, b):
+    """Whether two lists hold the same objects."""
+    return len(a) == len(b) and all(map(operator.is_, a, b))
+
+
 class AdamW(Optimizer):
     """Adam with decoupled weight decay and bias correction (t counts from 1):
 
@@ -485,7 +496,7 @@ class AdamW(Optimizer):
         for name in self.state_names:
             setattr(self, name, dict())
         self.masters = dict()
-        self._records = {}      # id(parameter) -> see _record
+        self._groups = {}       # see _update
         # the constants that the value tensors hold: see _refresh
         self._held = {a: (getattr(self, a), getattr(self, a).init_value,
                           getattr(self, v)) for a, v, _ in self._scheduled}
@@ -528,28 +539,24 @@ class AdamW(Optimizer):
             _eagerly(p.device, lambda: t.to_device(p.device))
         return t
 
-    def _record(self, name, p):
-        """What a step needs of a parameter beside its gradient: (parameter,
-        core tensor, core type, state key, its state tensors in the order of
-        ``_tables``)."""
-        core = p.data
-        if not core.is_contiguous():
-            raise ValueError("AdamW steps contiguous parameters")
-        key = self._state_key(name, p)
-        held = [self._state(n, key, p) for n in self.state_names]
-        if self.master_weights and p.dtype != tensor.float32:
-            held.append(self._slot(self.masters, key, p, tensor.float32,
-                                   copy=True))
-        r = self._records[id(p)] = (p, core, core.data_type(), name, key, held,
-                                    [t.data for t in held])
-        return r
-
-    def _tables(self, mixed):
-        return [getattr(self, n) for n in self.state_names] + \
-            ([self.masters] if mixed else [])
+    def _gather(self, names, params, mixed):
+        """The parameters' states, created on first use: (state keys, the
+        tensors of each table in the parameters' order)."""
+        for p in params:
+            if not p.data.is_contiguous():
+                raise ValueError("AdamW steps contiguous parameters")
+        keys = [self._state_key(n, p) for n, p in zip(names, params)]
+        columns = [[self._state(n, k, p) for k, p in zip(keys, params)]
+                   for n in self.state_names]
+        if mixed:
+            columns.append([self._slot(self.masters, k, p, tensor.float32,
+                                       copy=True)
+                            for k, p in zip(keys, params)])
+        return keys, columns
 
     def _update(self, items, scale):
-        lead = items[0][1]
+        names, params, grads = zip(*items)
+        lead = params[0]
         dev = lead.data.device()
         hypers = [t.data for t in (self.lr_value, self.decay_value,
                                    self.epsilon_value, self.beta_1_value,
@@ -557,24 +564,31 @@ class AdamW(Optimizer):
         if any(h.device() is not dev for h in hypers):
             self.device_check(lead, self.step_counter, *self._values())
         mixed = self.master_weights and lead.dtype != tensor.float32
-        tables = self._tables(mixed)
-        params, grads, states = [], [], []
-        for name, p, g in items:
-            r = self._records.get(id(p))
-            # the record holds while the parameter and its states are the
-            # tensors it was made of, on this device
-            if r is None or r[0] is not p or r[1] is not p.data or \
-                    r[2] != r[1]._dtype or r[3] != name or \
-                    len(r[5]) != len(tables) or \
-                    any([t.get(r[4]) is not h or h.data is not c or
-                         c._dev is not dev
-                         for t, h, c in zip(tables, r[5], r[6])]):
-                r = self._record(name, p)
-            params.append(r[1])
-            grads.append(g.data)
-            states.append(r[6])
-        singa.AdamWUpdateMulti(params, grads, states, mixed, hypers,
-                               self.state_bits, scale, self.seed)
+        # Looking the states of the same parameters up again is most of a small
+        # step's host work.  What was found holds while names, parameters and
+        # what the tables hold for them are the same objects, in place.
+        cores = list(map(_core, params))
+        group = (names, tuple(map(id, params)), mixed)
+        tables = [getattr(self, n) for n in self.state_names]
+        if mixed:
+            tables.append(self.masters)
+        found = self._groups.get(group)
+        if found is not None:
+            known, kept, keys, columns, states = found
+            if not (_same(known, cores) and all(
+                    _same(column, list(map(table.get, keys)))
+                    for table, column in zip(tables, columns)) and all(
+                    _same(was, list(map(_core, column)))
+                    for column, was in zip(columns, states)) and
+                    {dev} == set(map(_device, itertools.chain(*states)))):
+                found = None
+        if found is None:
+            keys, columns = self._gather(names, params, mixed)
+            states = [list(map(_core, column)) for column in columns]
+            # the parameters are kept with it: an id is theirs while they live
+            self._groups[group] = (cores, params, keys, columns, states)
+        singa.AdamWUpdateMulti(cores, list(map(_core, grads)), states, mixed,
+                               hypers, self.state_bits, scale, self.seed)
 
     sync_masters = SGD.sync_masters
     forget_masters = SGD.forget_masters

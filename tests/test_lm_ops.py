@@ -249,8 +249,13 @@ def test_rotary_zero_rows_and_empty(dev):
     want = turn64(rounded(g, "float32"), handle, torch.arange(2), True) * 1e3
     check(dx, want, scale=16 * E32 * 4e3)
     assert not got(dw).any()
-    y = autograd.rotary(handle, tensor.Tensor((2, 0, 3, 8), dev))
+    none = tensor.Tensor((2, 0, 3, 8), dev)
+    y = autograd.rotary(handle, none)
     assert y.shape == (2, 0, 3, 8)
+    op = autograd.Rotary(handle, norm=True)
+    op(none, put(dev, w))
+    dx, dw = op.backward(none.data)
+    assert dx.shape() == [2, 0, 3, 8] and not got(dw).any()
 
 
 def test_rotary_scalings():
@@ -299,6 +304,7 @@ def test_rotary_refusals(cpu_dev):
     for call, error in (
             (lambda: autograd.rotary(h, t(2, 3, 8)), ValueError),
             (lambda: autograd.rotary(h, t(2, 3, 4, 6)), ValueError),
+            (lambda: autograd.rotary(h, t(2, 3, 0, 8)), ValueError),
             (lambda: autograd.rotary(h, t(2, 3, 4, 8, dtype=tensor.int32)),
              TypeError),
             (lambda: autograd.rotary(h, x, t(3)), TypeError),
@@ -403,6 +409,22 @@ def test_token_log_prob_pieces(gpu_dev, rows):
     want, used = log_prob64(x, t)
     check(y, want, scale=rows_room(V) + 4 * E32 * 14)
     check_dx(op.backward(put(gpu_dev, dy).data), dy, x, t, used, "float16",
+             4 * E32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_token_log_prob_long_rows(gpu_dev, dtype):
+    """Rows that eight waves share, and a gradient that is stored past the
+    caches (over 128 MB)."""
+    rows, V = (700, 50257) if dtype == "float32" else (1400, 50257)
+    x, t = logits(rows, dtype, rows, V), labels(rows, V, rows)
+    dy = rounded(normal(7, rows), "float32")
+    op = autograd.TokenLogProb(put(gpu_dev, t))
+    y = op(put(gpu_dev, x, dtype))[0]
+    want, used = log_prob64(x, t)
+    check(y, want, scale=rows_room(V) + 4 * E32 * 14)
+    check_dx(op.backward(put(gpu_dev, dy).data), dy, x, t, used, dtype,
              4 * E32)
 
 
@@ -637,6 +659,7 @@ def test_loss_refusals(cpu_dev):
             (lambda: autograd.token_log_prob(x, t(3, 4, **i32)), ValueError),
             (lambda: autograd.token_log_prob(t(4, 0), t(4, **i32)),
              ValueError),
+            (lambda: autograd.token_log_prob(t(9), t(**i32)), ValueError),
             (lambda: autograd.preference_loss(x, lab, t(4)), ValueError),
             (lambda: autograd.preference_loss(x, lab, lab), TypeError),
             (lambda: autograd.preference_loss(t(3, 3, 9), t(3, 3, **i32),
@@ -727,17 +750,17 @@ def codes64(words, scales):
 
 def noise16(n, step, seed):
     """16 + 16 bits for each value: Philox4x32-10 in unsigned arithmetic."""
-    mask = 0xffffffff
-    out = np.empty((n + 3) // 4 * 4, np.int64)
-    for q in range((n + 3) // 4):
-        c, k = [q & mask, q >> 32, step, 0], [seed & mask, seed >> 32]
-        for _ in range(10):
-            a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
-            c = [(b >> 32) ^ c[1] ^ k[0], b & mask,
-                 (a >> 32) ^ c[3] ^ k[1], a & mask]
-            k = [(k[0] + 0x9E3779B9) & mask, (k[1] + 0xBB67AE85) & mask]
-        out[4 * q:4 * q + 4] = c
-    out = torch.from_numpy(out[:n])
+    u, low, half = np.uint64, np.uint64(0xffffffff), np.uint64(32)
+    q = np.arange((n + 3) // 4, dtype=np.uint64)
+    c = [q & low, q >> half, np.full_like(q, step), np.zeros_like(q)]
+    k = [seed & 0xffffffff, seed >> 32]
+    for _ in range(10):
+        a, b = u(0xD2511F53) * c[0], u(0xCD9E8D57) * c[2]
+        c = [(b >> half) ^ c[1] ^ u(k[0]), b & low,
+             (a >> half) ^ c[3] ^ u(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xffffffff,
+             (k[1] + 0xBB67AE85) & 0xffffffff]
+    out = torch.from_numpy(np.stack(c, 1).reshape(-1)[:n].astype(np.int64))
     return (out & 0xffff).double() / 65536, (out >> 16).double() / 65536
 
 
@@ -887,6 +910,68 @@ def test_adamw_schedule_states_and_masters(dev):
         assert (got(p) == rounded(got(o.masters["w"]), "float16")).all()
 
 
+def test_adamw_follows_its_tables(dev):
+    """A step reads the states that the tables hold now: masters dropped or
+    overwritten, states loaded in place or put in anew."""
+    o = opt.AdamW(lr=0.1, weight_decay=0.0)
+    p, g = put(dev, normal(1, 300), "float16"), put(dev, normal(2, 300),
+                                                    "float16")
+    p.name = "w"
+    o.apply_many([(p, g)])
+    o.forget_masters()
+    p.copy_from_numpy(np.full(300, 5.0, np.float16))
+    o.apply_many([(p, g)])
+    assert (got(p) - 5.0).abs().max() < 0.5
+    p.copy_from_numpy(np.full(300, -5.0, np.float16))
+    o.sync_masters({"w": p})
+    o.apply_many([(p, g)])
+    assert (got(p) + 5.0).abs().max() < 0.5
+    zero = put(dev, torch.zeros(300, dtype=torch.float64))
+    for fresh in (False, True):
+        o.apply_many([(p, g)])
+        if fresh:
+            o.m["w"] = zero.clone()
+        else:
+            o.set_states(dict(o.get_states(), m={"w": zero}))
+        o.apply_many([(p, g)])
+        check(o.m["w"], got(g) * 0.1, scale=4 * E32)
+    # another tensor in the parameter's place: the same name, its own state
+    q = put(dev, normal(1, 20))
+    q.name = "w"
+    o.apply_many([(q, put(dev, normal(2, 20)))])
+    assert got(o.m["w"]).numel() == 300 and len(o.m) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_large_step(gpu_dev, bits):
+    """Large enough to go past the caches; whole chunks and a ragged end."""
+    o = opt.AdamW(**HYPER, state_bits=bits, seed=9)
+    n = [5_000_003, 4_100_000]
+    start = [rounded(normal(i, k), "float32") for i, k in enumerate(n)]
+    grads = [rounded(normal(9 + i, k), "float32") for i, k in enumerate(n)]
+    params = [put(gpu_dev, p) for p in start]
+    for i, p in enumerate(params):
+        p.name = "w%d" % i
+    o.apply_many([(p, put(gpu_dev, g)) for p, g in zip(params, grads)])
+    for i, g in enumerate(grads):
+        zero = torch.zeros_like(g)
+        p64, m, v = adamw64(start[i], g, zero, zero, 1)
+        check(params[i], p64, scale=16 * E32 * F32["lr"] * 10 +
+              3 * E32 * p64.abs())
+        key = "w%d" % i
+        if bits == 32:
+            check(o.m[key], m, scale=16 * E32)
+            check(o.v[key], v, scale=64 * E32)
+            continue
+        um, ur = noise16(n[i], 0, 9)
+        for words, scales, x, u, keep in (
+                (o.m, o.m_scale, m, um, False),
+                (o.r, o.r_scale, torch.sqrt(v), ur, True)):
+            _, c, s = codes64(words[key], scales[key])
+            check_codes(c, s, x, u, keep)
+
+
 def test_adamw_refusals(cpu_dev):
     with pytest.raises(ValueError):
         opt.AdamW(state_bits=4)
@@ -908,6 +993,10 @@ def test_adamw_refusals(cpu_dev):
     o.set_states(states)
     with pytest.raises(ValueError):
         o.apply_many([(p, g)])
+    # one launch steps its tensors side by side: the same memory only once
+    for twice in (p, p.copy()):
+        with pytest.raises(ValueError):
+            opt.AdamW().apply_many([(p, g), (twice, g)])
     q = put(cpu_dev, normal(1, 4, 5)).transpose()
     q.name = "q"
     with pytest.raises(ValueError):
@@ -1047,6 +1136,92 @@ def test_another_stream(gpu_dev):
     s.synchronize()
     check(y, rotary64(x, None, handle, torch.arange(50), 0), scale=24 * E32 * 6)
     check(z, log_prob64(lg, lab)[0], scale=rows_room(5000) + 64 * E32)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(gpu_dev):
+    """More than 2^31 values in one tensor: its first and last rows."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB of device memory")
+
+    def raw(*shape, dtype=tensor.bfloat16):
+        t = tensor.Tensor(shape, gpu_dev, dtype)
+        return t, t.data.view()
+
+    # losses
+    V, rows = 50257, 43000
+    x, vx = raw(rows, V)
+    t, vt = raw(rows, dtype=tensor.int32)
+    dy, vd = raw(rows, dtype=tensor.float32)
+    vx.zero_()
+    vt.fill_(-1)
+    vd.fill_(0.5)
+    ends = [0, 1, rows - 2, rows - 1]
+    some = logits(1, "bfloat16", 4, V)
+    lab = torch.tensor([3, V - 1, 0, V - 1])
+    vx[ends] = some.to(vx)
+    vt[ends] = lab.to(vt)
+    op = autograd.TokenLogProb(t)
+    y = op(x)[0].data.view()
+    want, used = log_prob64(some, lab)
+    assert ((y[ends].double().cpu() - want).abs() <=
+            rows_room(V) + 64 * E32).all()
+    dx = op.backward(dy.data).view()
+    check_dx(tensor.Tensor(device=device.get_default_device(),
+                           data=dx[ends].float().cpu().numpy()),
+             torch.full((4,), 0.5, dtype=torch.float64), some, lab, used,
+             "bfloat16", 4 * E32)
+    assert not dx[2:rows - 2].any()
+    del x, vx, dx, op
+    # rotary: 2^31 + 2^13 values
+    S, H, D = (1 << 19) + 2, 32, 128
+    handle = singa_wrap.RotaryHandle(D)
+    x, vx = raw(1, S, H, D)
+    vx.fill_(1.0)
+    y = autograd.rotary(handle, x).data.view()
+    for s in (0, 1, S - 2, S - 1):
+        want = turn64(torch.ones(1, 1, 1, D, dtype=torch.float64), handle,
+                      torch.tensor([s]))
+        off = (y[0, s].double().cpu() - want[0, 0]).abs()
+        assert (off <= HALF["bfloat16"] * want[0, 0].abs() + 24 * E32).all()
+    del x, vx, y
+    # AdamW, 8 bits: the last of 2^31 + 300 elements
+    n = (1 << 31) + 300
+    p, vp = raw(n)
+    g, vg = raw(n)
+    vp.fill_(1.0)
+    vg.fill_(0.25)
+    p.name = "w"
+    o = opt.AdamW(lr=0.5, weight_decay=0.0, state_bits=8, master_weights=False)
+    o.apply_many([(p, g)])
+    # every first step is lr long: 1 - 0.5
+    for part in (vp[:300], vp[(1 << 31) - 5:]):
+        assert ((part.double() - 0.5).abs() <= HALF["bfloat16"]).all()
+    words = o.m["w"].data.view()
+    # the largest of every block is its scale times 448, code 0x7e; where the
+    # product falls a rounding short and the noise is 0 (of 2^16) the code below
+    whole = (words == 0x7e7e7e7e).sum().item()
+    assert n // 4 * (1 - 2.0 ** -13) < whole <= n // 4
+
+
+@pytest.mark.gpu
+def test_operands_of_another_device_are_refused(gpu_dev, cpu_dev):
+    h = singa_wrap.RotaryHandle(8)
+    x = tensor.Tensor((1, 2, 3, 8), gpu_dev)
+    lg = tensor.Tensor((2, 9), gpu_dev)
+    lab = tensor.Tensor((2,), gpu_dev, tensor.int32)
+    f = tensor.Tensor((2,), cpu_dev)
+    for call in (
+            lambda: autograd.rotary(h, x, tensor.Tensor((2,), cpu_dev,
+                                                        tensor.int32)),
+            lambda: autograd.rotary(h, x, scale=tensor.Tensor((8,), cpu_dev)),
+            lambda: autograd.token_log_prob(lg, tensor.Tensor(
+                (2,), cpu_dev, tensor.int32)),
+            lambda: autograd.policy_loss(lg, lab, f, f),
+            lambda: opt.AdamW().apply_many([(lg, tensor.Tensor((2, 9),
+                                                               cpu_dev))])):
+        with pytest.raises(ValueError):
+            call()
 
 
 @pytest.mark.gpu
