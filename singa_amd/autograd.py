@@ -199,24 +199,24 @@ class Operator(object):
                 "%s takes Tensors, got %s" % (self.name, type(x).__name__))
         # inputs whose gradient nobody consumes (data fed to the network):
         # ops may return None for them instead of computing it
-        self.x_needs_grad = tuple(
+        self.x_needs_grad = tuple([
             x.stores_grad or
             (x.requires_grad and not isinstance(x.creator, Dummy))
-            for x in xs)
+            for x in xs])
         # an op fed only by such inputs has nothing to back-propagate, and
         # neither has anything computed from its outputs alone (e.g. an
         # attention mask derived from the input ids)
         self.requires_grad = any(self.x_needs_grad)
         self.src = [(x.creator, x.uid, x if x.stores_grad else None,
                      x.stores_grad) for x in xs]
-        produced = self.forward(*(x.data for x in xs))
+        produced = self.forward(*[x.data for x in xs])
         if not isinstance(produced, tuple):
             produced = (produced,)
-        ys = tuple(
+        ys = tuple([
             Tensor(device=core.device(), data=core, creator=self,
                    requires_grad=self.requires_grad,
                    name=self.output_name(i))
-            for i, core in enumerate(produced))
+            for i, core in enumerate(produced)])
         self.y_id2idx = {y.uid: i for i, y in enumerate(ys)}
         return ys
 

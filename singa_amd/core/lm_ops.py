@@ -180,20 +180,22 @@ def _rotary(name, handle, xs, scales, positions, eps, dys):
     dws = [Tensor(w._shape, dev, w._dtype) for w in scales] if back else []
     at = [positions] if positions is not None else []
     reads = inputs + grads + scales + at
-    ends = []
-    for group in (inputs, grads, scales, at, ys):
-        ends.append((ends[-1] if ends else 0) + len(group))
-
-    def body(*ts):
-        i, g, w, p, y = ends
-        dev.math.rotary(handle, ts[:i], ts[i:g], ts[g:w],
-                        ts[w] if p > w else None, ts[p:y], ts[y:], eps)
-
     _one_device(name, dev, reads)
     if xs[0].Size() == 0:
         for w in dws:      # sums over nothing
             w.SetFloatValue(0.0)
+    elif not dev.graph_enabled():
+        dev.math.rotary(handle, inputs, grads, scales, positions, ys, dws, eps)
     else:
+        ends = []
+        for group in (inputs, grads, scales, at, ys):
+            ends.append((ends[-1] if ends else 0) + len(group))
+
+        def body(*ts):
+            i, g, w, p, y = ends
+            dev.math.rotary(handle, ts[:i], ts[i:g], ts[g:w],
+                            ts[w] if p > w else None, ts[p:y], ts[y:], eps)
+
         _submit(dev, name, body, reads, ys + dws)
     return ys, dws
 
@@ -228,45 +230,51 @@ class TokenLoss(object):
                  kl=0.0):
         _float_operand("logits", x)
         _int_operand("a label", label)
-        _refuse(x.nDim() < 2 or x._shape[:-1] != label._shape,
-                "logits %s need labels %s, got %s", tuple(x._shape),
-                tuple(x._shape[:-1]), tuple(label._shape))
-        _refuse(x._shape[-1] < 1, "an empty vocabulary")
+        shape = label._shape
+        if len(x._shape) < 2 or x._shape[:-1] != shape:
+            raise ValueError("logits %s need labels %s, got %s" % (
+                tuple(x._shape), tuple(x._shape[:-1]), tuple(shape)))
+        self.V = x._shape[-1]
+        _refuse(self.V < 1, "an empty vocabulary")
         self.mode = mode
         self.pairs = self.seq = 0
         if mode == LOSS_PREFERENCE:
-            _refuse(x.nDim() != 3 or x._shape[0] % 2 or x.Size() == 0,
+            if len(x._shape) != 3 or shape[0] % 2 or not all(shape):
+                raise ValueError(
                     "preference logits are (2 pairs, sequence, vocabulary), "
-                    "the chosen ones first, got %s", tuple(x._shape))
-            self.pairs, self.seq = x._shape[0] // 2, x._shape[1]
+                    "the chosen ones first, got %s" % (tuple(x._shape),))
+            self.pairs, self.seq = shape[0] // 2, shape[1]
+        given = []
         for what, t in (("reference", ref), ("old", old), ("advantages", adv),
                         ("weights", weight)):
             if t is not None:
                 _float_operand(what, t)
-                _refuse(t._shape != label._shape,
-                        "%s have the labels' shape %s, got %s", what,
-                        tuple(label._shape), tuple(t._shape))
-        _one_device("a token loss", x._dev,
-                    [t for t in (label, ref, old, adv, weight)
-                     if t is not None])
+                if t._shape != shape:
+                    raise ValueError("%s have the labels' shape %s, got %s" % (
+                        what, tuple(shape), tuple(t._shape)))
+                if t._dtype != dtypes.kFloat32:
+                    t = t.AsType(dtypes.kFloat32)
+                t = Contiguous(t)
+            given.append(t)
+        self.extra = given
         self.x, self.label = Contiguous(x), Contiguous(label)
-        self.extra = [t if t is None else
-                      Contiguous(t.AsType(dtypes.kFloat32))
-                      for t in (ref, old, adv, weight)]
+        _one_device("a token loss", x._dev, [self.label] +
+                    [t for t in given if t is not None])
         self.consts = (float(beta), float(smoothing), 1.0 - float(clip[0]),
                        1.0 + float(clip[1]), float(kl))
-        self.V = x._shape[-1]
-        self.rows = x.Size() // self.V
+        self.rows = 1
+        for n in shape:
+            self.rows *= n
 
     def forward(self):
         """-> the loss (1,) or, for the log-probabilities, (labels' shape);
         float32."""
         dev, rows, f32 = self.x._dev, self.rows, dtypes.kFloat32
         logp = self.mode == LOSS_LOG_PROB
-        # the result of each row is the log-probabilities' output, else kept
-        # of each row the largest logit and the log of the sum relative to it,
-        # then the derivative (policy), then what rows' derivatives are
-        # multiplied by (policy: one number, preference: one for each pair)
+        # kept of each row: the largest logit, the log of the sum relative to
+        # it, the row's result (unless that is the output), its derivative
+        # (policy); then what rows' derivatives are multiplied by (policy: one
+        # number, preference: one for each pair)
         n = {LOSS_LOG_PROB: 2 * rows, LOSS_PREFERENCE: 3 * rows + self.pairs,
              LOSS_POLICY: 4 * rows + 1}[self.mode]
         self.saved = Tensor([n], dev, f32)
@@ -283,7 +291,8 @@ class TokenLoss(object):
             dev.math.token_loss_fwd(spec, flat[0], flat[1], extra, flat[-2],
                                     flat[-1])
 
-        _submit(dev, "TokenLossForward", body, ins, [self.saved, loss])
+        if self.rows or not logp:
+            _submit(dev, "TokenLossForward", body, ins, [self.saved, loss])
         return loss
 
     def backward(self, dy):
@@ -311,7 +320,8 @@ class TokenLoss(object):
 
         reads = [self.x, self.label, self.saved] + weight + dys
         _one_device("TokenLossBackward", dev, reads)
-        _submit(dev, "TokenLossBackward", body, reads, [dx])
+        if self.rows:
+            _submit(dev, "TokenLossBackward", body, reads, [dx])
         return dx
 
 
@@ -327,40 +337,60 @@ _held_in = operator.attrgetter("_block")
 _placed = operator.attrgetter("_dev")
 
 
-def AdamWUpdateMulti(params, grads, states, mixed, hypers, state_bits=32,
-                     scale=1.0, seed=0):
-    """One AdamW step for a list of contiguous parameters of one type (one
-    graph node, one launch for every 48 tensors).  states: lists of the
-    parameters' states, (m, v) -- float32, of the parameter's shape -- or, with
-    state_bits 8, (m, r, m_scale, r_scale): int32 words of four e4m3 codes of
-    the first moment and of the root of the second, in whole blocks of 256
-    values, and a float32 scale for each block; behind them, when ``mixed``,
-    the float32 master copies of 16-bit parameters.  hypers = (lr,
-    weight_decay, epsilon, beta_1, beta_2, step): one-element float32
-    tensors."""
-    dev, n, dtype = params[0]._dev, len(params), params[0]._dtype
-    # the tensors of a launch are stepped side by side
-    _refuse(len(set(map(id, map(_held_in, params)))) != n,
-            "a parameter twice in one step")
-    if {dtype} != set(map(_typed, grads)):
-        grads = [g.AsType(dtype) for g in grads]
-    grads = [g if g._stride == p._stride else Contiguous(g)
-             for p, g in zip(params, grads)]
+class AdamWGroup(object):
+    """Parameters of one type, contiguous, and their states.  states: lists of
+    the parameters' (m, v) -- float32, of the parameter's shape -- or, with 8
+    bits, (m, r, m_scale, r_scale): int32 words of four e4m3 codes of the first
+    moment and of the root of the second, in whole blocks of 256 values, and a
+    float32 scale for each block; behind them, when ``mixed``, the float32
+    master copies of 16-bit parameters.  It holds while every tensor in it
+    keeps its storage (``storage``: parameters, then each list of states)."""
+
+    def __init__(self, params, states, mixed):
+        self.params, self.states = params, states
+        self.mixed = bool(mixed)
+        self.dev, self.dtype = params[0]._dev, params[0]._dtype
+        n = len(params)
+        # the tensors of a launch are stepped side by side
+        _refuse(len(set(map(id, map(_held_in, params)))) != n,
+                "a parameter twice in one step")
+        self.members = [*params, *itertools.chain(*states)]
+        _one_device("AdamWUpdateMulti", self.dev, self.members)
+        self.sizes = [p.Size() for p in params]
+        self.strides = [p._stride for p in params]
+        self.storage = [t._storage() for t in self.members]
+        self.columns = [self.storage[i:i + n]
+                        for i in range(0, len(self.storage), n)]
+        self.addresses = [[t.data_ptr() for t in c] for c in self.columns]
+
+
+def AdamWUpdateMulti(group, grads, hypers, state_bits=32, scale=1.0, seed=0):
+    """One AdamW step of an AdamWGroup (one graph node, one launch for every
+    48 parameters).  hypers = (lr, weight_decay, epsilon, beta_1, beta_2,
+    step): one-element float32 tensors."""
+    dev, n = group.dev, len(group.params)
+    if {group.dtype} != set(map(_typed, grads)):
+        grads = [g.AsType(group.dtype) for g in grads]
+    grads = [g if g._stride == s else Contiguous(g)
+             for g, s in zip(grads, group.strides)]
+    if {dev} != set(map(_placed, itertools.chain(grads, hypers))):
+        _one_device("AdamWUpdateMulti", dev, [*grads, *hypers])
     scale, seed, state_bits = float(scale), int(seed), int(state_bits)
-    reads = [*params, *grads, *itertools.chain(*states), *hypers]
-    if {dev} != set(map(_placed, reads)):
-        _one_device("AdamWUpdateMulti", dev, reads)
-    sizes = [p.Size() for p in params]
-    columns = 2 + len(states)
+    if not dev.graph_enabled():
+        flat = [t._storage() for t in hypers]
+        dev.math.adamw_update_multi(
+            group.sizes, group.columns, [g._storage() for g in grads],
+            group.mixed, flat, state_bits, scale, seed, group.addresses)
+        return
+    sizes, mixed = group.sizes, group.mixed
 
     def body(*ts):
         # the outputs stand behind the inputs: they are the same blocks
-        flat = list(map(_stored, ts[:columns * n + 6]))
-        flat = [t._storage() if s is None else s for t, s in zip(ts, flat)]
+        flat = [t._storage() for t in ts[:len(group.members) + n + 6]]
+        grads, flat = flat[:n], flat[n:]
         dev.math.adamw_update_multi(
-            sizes, [flat[i * n:(i + 1) * n] for i in range(columns)],
-            bool(mixed), flat[columns * n:], state_bits, scale, seed)
+            sizes, [flat[i:i + n] for i in range(0, len(flat) - 6, n)], grads,
+            mixed, flat[-6:], state_bits, scale, seed)
 
-    _submit(dev, "AdamWUpdateMulti", body, reads,
-            [*params, *itertools.chain(*states)])
-    return params
+    _submit(dev, "AdamWUpdateMulti", body, [*grads, *group.members, *hypers],
+            group.members)

@@ -475,10 +475,10 @@ class CpuMath(object):
             p.copy_(pv - lr * upd)
 
     # ---- AdamW (same contract as the HIP backend) --------------------------------
-    def adamw_update_multi(self, sizes, columns, mixed, hypers, state_bits,
-                           scale, seed):
-        ps, gs, s1, s2 = columns[:4]
-        sc1, sc2 = columns[4:6] if state_bits == 8 else (None, None)
+    def adamw_update_multi(self, sizes, columns, gs, mixed, hypers, state_bits,
+                           scale, seed, addresses=None):
+        ps, s1, s2 = columns[:3]
+        sc1, sc2 = columns[3:5] if state_bits == 8 else (None, None)
         masters = columns[-1] if mixed else None
         one = np.float32(1.0)
         lr, wd, eps, b1, b2 = (np.float32(t.reshape(-1)[0].item())

@@ -1768,19 +1768,20 @@ class HipMath(object):
             [p.numel() for p in ps], ptr[0], ptr[1], ptr[2], ptr[3], ptr[4],
             ptr[5], float(scale), self._s())
 
-    def adamw_update_multi(self, sizes, columns, mixed, hypers, state_bits,
-                           scale, seed):
+    def adamw_update_multi(self, sizes, columns, grads, mixed, hypers,
+                           state_bits, scale, seed, addresses=None):
         """One AdamW step on flat tensors, one launch per 48 parameters.
-        columns: lists of the parameters, gradients, states (in the order of
-        lm_ops.AdamWUpdateMulti) and, when ``mixed``, float masters."""
-        at = [list(map(torch.Tensor.data_ptr, c)) for c in columns]
-        master = at.pop() if mixed else []
-        if state_bits == 32:
-            at += [[], []]
+        columns: lists of the parameters, the states (lm_ops.AdamWGroup) and,
+        when ``mixed``, the float masters; addresses: theirs, where known."""
+        address = torch.Tensor.data_ptr
+        at = addresses or [list(map(address, c)) for c in columns]
+        at, master = (at[:-1], at[-1]) if mixed else (at, [])
+        scales = at[3:] if state_bits == 8 else ([], [])
         with self._current():
             self.k.adamw_update_multi(
-                _code(columns[0][0]), state_bits, at[0], at[1], master,
-                *at[2:], sizes, *[t.data_ptr() for t in hypers], scale,
+                _code(columns[0][0]), state_bits, at[0],
+                list(map(address, grads)), master, at[1], at[2], *scales,
+                sizes, *map(address, hypers), scale,
                 seed & 0xffffffffffffffff, self._s())
 
     # ---- rotary positions ---------------------------------------------------------

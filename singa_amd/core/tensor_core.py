@@ -60,14 +60,18 @@ class Tensor(object):
             if self._block is not None:
                 self._block.IncRefCount()
             return
-        if shape is None:
-            shape = []
-        self._shape = [int(s) for s in shape]
-        self._stride = _contig_strides(self._shape)
+        self._shape = list(map(int, shape)) if shape is not None else []
+        # strides and size in one pass: every operator makes tensors
+        stride, n = [], 1
+        for s in reversed(self._shape):
+            stride.append(n)
+            n *= s
+        stride.reverse()
+        self._stride = stride
         self._dtype = int(dtype)
         self._dev = device if device is not None else get_default_device()
-        n = Product(self._shape)
-        self._block = self._dev.NewBlock(n * dtypes.SizeOf(self._dtype))
+        self._block = self._dev.NewBlock(
+            n * dtypes.SizeOf(self._dtype) if stride else 0)
         self._block.IncRefCount()
 
     def __del__(self):

@@ -450,7 +450,9 @@ class Adam(_Adaptive):
 
 
 _core = operator.attrgetter("data")
-_device = operator.attrgetter("_dev")
+_dtype = operator.attrgetter("dtype")
+_place = operator.attrgetter("device")
+_storage_of = operator.attrgetter("data._block.data")
 
 
 def _same(a, b):
@@ -554,41 +556,59 @@ class AdamW(Optimizer):
                             for k, p in zip(keys, params)])
         return keys, columns
 
+    def apply_many(self, pairs, scale=1.0):
+        """As every optimizer's; parameters of one type on one device, the
+        ordinary case, are told by a few looks over the whole list."""
+        pairs = list(pairs)
+        if not pairs:
+            return
+        params, grads = zip(*pairs)
+        if len(set(map(_dtype, params))) > 1 or \
+                len(set(map(id, map(_place, params)))) > 1:
+            return super(AdamW, self).apply_many(pairs, scale)
+        for p, g in zip(params, grads):
+            assert p.shape == g.shape, ("shape mismatch", p.shape, g.shape)
+        self._step(tuple(map(_name_of, params)), params, grads, scale)
+
     def _update(self, items, scale):
-        names, params, grads = zip(*items)
+        self._step(*zip(*items), scale)
+
+    def _step(self, names, params, grads, scale):
         lead = params[0]
         dev = lead.data.device()
         hypers = [t.data for t in (self.lr_value, self.decay_value,
                                    self.epsilon_value, self.beta_1_value,
                                    self.beta_2_value, self.step_counter)]
-        if any(h.device() is not dev for h in hypers):
+        if any([h._dev is not dev for h in hypers]):
             self.device_check(lead, self.step_counter, *self._values())
         mixed = self.master_weights and lead.dtype != tensor.float32
         # Looking the states of the same parameters up again is most of a small
-        # step's host work.  What was found holds while names, parameters and
-        # what the tables hold for them are the same objects, in place.
-        cores = list(map(_core, params))
-        group = (names, tuple(map(id, params)), mixed)
+        # step's host work.  What was found holds while names and parameters
+        # are the same, the tables hold the same tensors for them and all have
+        # their storage (a tensor that changes type, size or place gets
+        # another).
+        at = (names, tuple(map(id, params)), mixed)
         tables = [getattr(self, n) for n in self.state_names]
         if mixed:
             tables.append(self.masters)
-        found = self._groups.get(group)
+        found = self._groups.get(at)
         if found is not None:
-            known, kept, keys, columns, states = found
-            if not (_same(known, cores) and all(
-                    _same(column, list(map(table.get, keys)))
-                    for table, column in zip(tables, columns)) and all(
-                    _same(was, list(map(_core, column)))
-                    for column, was in zip(columns, states)) and
-                    {dev} == set(map(_device, itertools.chain(*states)))):
+            group, kept, keys, columns = found
+            if not (_same(group.params, list(map(_core, params))) and
+                    all([_same(column, list(map(table.get, keys)))
+                         for table, column in zip(tables, columns)]) and
+                    _same(group.storage, list(map(_storage_of, itertools.chain(
+                        params, *columns))))):
                 found = None
         if found is None:
             keys, columns = self._gather(names, params, mixed)
-            states = [list(map(_core, column)) for column in columns]
+            group = singa.AdamWGroup(list(map(_core, params)),
+                                     [list(map(_core, c)) for c in columns],
+                                     mixed)
             # the parameters are kept with it: an id is theirs while they live
-            self._groups[group] = (cores, params, keys, columns, states)
-        singa.AdamWUpdateMulti(cores, list(map(_core, grads)), states, mixed,
-                               hypers, self.state_bits, scale, self.seed)
+            self._groups[at] = (group, params, keys, columns)
+        singa.AdamWUpdateMulti(group, list(map(_core, grads)), hypers,
+                               self.state_bits, scale, self.seed)
 
     sync_masters = SGD.sync_masters
     forget_masters = SGD.forget_masters

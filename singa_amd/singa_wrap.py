@@ -19,7 +19,7 @@ from .core.nn_ops import *  # noqa: F401,F403
 from .core.rnn_ops import *  # noqa: F401,F403
 from .core.lm_ops import (RotaryHandle, RotaryForward, RotaryBackward,
                           TokenLoss, LOSS_LOG_PROB, LOSS_PREFERENCE,
-                          LOSS_POLICY, AdamWUpdateMulti, ADAMW_BLOCK)
+                          LOSS_POLICY, AdamWGroup, AdamWUpdateMulti, ADAMW_BLOCK)
 from .parallel.communicator import Communicator, NcclIdHolder
 
 CudaGPU = HipGPU

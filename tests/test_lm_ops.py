@@ -619,9 +619,13 @@ def test_nothing_takes_part(dev):
         op = autograd.PolicyLoss(lab, nan, nan, w, nan, kl=0.1)
         assert float(got(op(x)[0])) == 0.0
         assert not got(op.backward(1.0)).any()
-    y = autograd.token_log_prob(tensor.Tensor((0, 5), dev),
-                                tensor.Tensor((0,), dev, tensor.int32))
-    assert y.shape == (0,)
+    none, no = tensor.Tensor((0, 5), dev), tensor.Tensor((0,), dev)
+    op = autograd.TokenLogProb(tensor.Tensor((0,), dev, tensor.int32))
+    assert op(none)[0].shape == (0,)
+    assert op.backward(no.data).shape() == [0, 5]
+    op = autograd.PolicyLoss(tensor.Tensor((0,), dev, tensor.int32), no, no)
+    assert float(got(op(none)[0])) == 0.0
+    assert op.backward(1.0).shape() == [0, 5]
 
 
 def test_losses_through_the_tape(dev):
@@ -935,6 +939,17 @@ def test_adamw_follows_its_tables(dev):
             o.set_states(dict(o.get_states(), m={"w": zero}))
         o.apply_many([(p, g)])
         check(o.m["w"], got(g) * 0.1, scale=4 * E32)
+    # a state moved or converted under the optimizer's hands
+    o.v["w"].to_type(tensor.float16)
+    with pytest.raises(ValueError):
+        o.apply_many([(p, g)])
+    o.v["w"] = zero.clone()
+    o.apply_many([(p, g)])
+    # a parameter that grew has states of the wrong size
+    p.data.Resize([400])
+    p.shape = (400,)
+    with pytest.raises(ValueError):
+        o.apply_many([(p, put(dev, normal(2, 400), "float16"))])
     # another tensor in the parameter's place: the same name, its own state
     q = put(dev, normal(1, 20))
     q.name = "w"
