@@ -1824,10 +1824,11 @@ class HipMath(object):
         at, row = saved.data_ptr(), 4 * rows
         pieces = self.k.token_loss_pieces(rows, V)
         part = self._tmp(2 * rows * pieces) if pieces > 1 else None
-        sums = self._tmp(2 * pairs, torch.float64) if pairs else None
+        words = self.k.token_loss_sums(mode, rows, pairs) if mode else 0
+        sums = self._tmp(words, torch.float64) if words else None
         where = (at, at + row, at + 2 * row if mode else out.data_ptr(),
                  at + 3 * row, at + (4 if mode == 2 else 3) * row,
-                 sums.data_ptr() if pairs else 0,
+                 sums.data_ptr() if words else 0,
                  part.data_ptr() if pieces > 1 else 0)
         with self._current():
             self.k.token_loss_fwd(

@@ -859,7 +859,8 @@ PYBIND11_MODULE(_hip, m) {
 
   // ---- losses over token log-probabilities -------------------------------------
   m.def("token_loss_pieces", &sa_token_loss_pieces);
-  // saved: (top, norm, value, coef, total, seq_sum, part) addresses
+  m.def("token_loss_sums", &sa_token_loss_sums);
+  // saved: (top, norm, value, coef, total, sums, part) addresses
   m.def("token_loss_fwd", [](int dt, int mode, uintptr_t x, uintptr_t label,
                              int64_t rows, int64_t V, int64_t pairs,
                              int64_t seq, uintptr_t ref, uintptr_t old,
@@ -876,7 +877,7 @@ PYBIND11_MODULE(_hip, m) {
     d.clip_hi = consts[3]; d.kl = consts[4];
     d.top = (float *)P(saved[0]); d.norm = (float *)P(saved[1]);
     d.value = (float *)P(saved[2]); d.coef = (float *)P(saved[3]);
-    d.total = (float *)P(saved[4]); d.seq_sum = (double *)P(saved[5]);
+    d.total = (float *)P(saved[4]); d.sums = (double *)P(saved[5]);
     d.part = (float2 *)P(saved[6]);
     d.loss = (float *)P(loss);
     check(sa_token_loss_fwd(dt, &d, S(s)), "token_loss_fwd");

@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // values under one scale: four for each lane
+constexpr int64_t kLaunchChunks = (1 << 24) - 1;
 
 struct Consts {
   float lr, decay, eps, b1, k1, b2, k2, c1, c2, root_c2, scale;
@@ -449,8 +450,9 @@ int sa_adamw_update_multi(int dtype, int state_bits, int count, void *const *p,
     for (; k < kAdamwMaxTensors && first + k < count; ++k) {
       const int i = first + k;
       const int64_t mine = (n[i] + kAdamwChunk - 1) / kAdamwChunk;
-      if (mine > 0x7fffffff) return -2;
-      if (chunks + mine > 0x7fffffff) break;   // the rest in the next launch
+      // a launch counts its threads in 32 bits
+      if (mine > kLaunchChunks) return -2;
+      if (chunks + mine > kLaunchChunks) break;   // the rest in the next one
       b.p[k] = p[i];
       b.g[k] = g[i];
       b.master[k] = master ? master[i] : nullptr;

@@ -443,17 +443,19 @@ struct TokenLossDesc {
   float *top = nullptr, *norm = nullptr, *value = nullptr;
   float *coef = nullptr;            // policy: (rows)
   float *total = nullptr;           // preference: (pairs), policy: (1)
-  double *seq_sum = nullptr;        // preference: (2 pairs)
+  double *sums = nullptr;           // sa_token_loss_sums words
   float *loss = nullptr;            // (1)
   float2 *part = nullptr;           // (rows, pieces) where pieces > 1
   const float *dy = nullptr;        // log-prob: (rows), else (1) or null for 1
   float dy_scale = 1.f;
   void *dx = nullptr;               // (rows, V)
-  int64_t piece = 0;                // set by the launcher
+  int64_t piece = 0, first = 0;     // set by the launcher
 };
 }  // namespace sa
 // workgroups the launcher takes for each row
 int sa_token_loss_pieces(int64_t rows, int64_t V);
+// float64 words of scratch that the forward pass needs
+int64_t sa_token_loss_sums(int mode, int64_t rows, int64_t pairs);
 int sa_token_loss_fwd(int dtype, const sa::TokenLossDesc *d, hipStream_t s);
 int sa_token_loss_bwd(int dtype, const sa::TokenLossDesc *d, hipStream_t s);
 

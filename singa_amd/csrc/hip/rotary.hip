@@ -442,6 +442,8 @@ static int rotary_run(int dtype, const RotaryDesc *d, bool bwd, hipStream_t s) {
     while (tile > 1 && a.tokens / tile < 512) tile >>= 1;
     p.tile = tile;
     p.blocks = (a.tokens + tile - 1) / tile;
+    // (a launch counts its threads in 32 bits; workgroups stride over the tiles)
+    if (p.blocks > 1 << 22) p.blocks = 1 << 22;
     if (sums && p.blocks > kRotaryMaxBlocks) p.blocks = kRotaryMaxBlocks;
     grid += p.blocks;
   }

@@ -196,7 +196,8 @@ template <typename T, int VEC, int WPR>
 __global__ void __launch_bounds__(threads_of(WPR))
     token_rows_kernel(TokenLossDesc d) {
   const int wave = threadIdx.x >> 6;
-  const int64_t r = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  const int64_t r =
+      d.first + (WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x);
   const bool used = r < d.rows && takes_part(d, r);
   Running run;
   if (used) {
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(threads_of(WPR))
 template <typename T>
 __global__ void __launch_bounds__(64)
     token_join_kernel(TokenLossDesc d, int pieces) {
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.x;   // few rows: one launch
   const bool used = takes_part(d, r);
   Running run;
   if (used) {
@@ -263,16 +264,43 @@ __device__ __forceinline__ double soft_plus(double v) {
   return fmax(v, 0.0) + log1p(exp(-fabs(v)));
 }
 
-// One workgroup adds up what the rows left: the rows' own work is V times
-// larger.
-__global__ void __launch_bounds__(1024) policy_total_kernel(TokenLossDesc d) {
-  double loss = 0.0, total = 0.0;
+// What the rows left is added up by one workgroup up to kOneBlockRows rows (16
+// loads for each thread and value, 4 to 5 us), above that by many first.
+constexpr int64_t kOneBlockRows = 32768;
+constexpr int kParts = 256;
+
+// loss and weight of every `step`-th row
+__device__ __forceinline__ void add_rows(const TokenLossDesc &d, int64_t first,
+                                         int64_t step, double &loss,
+                                         double &total) {
 #pragma unroll 4
-  for (int64_t r = threadIdx.x; r < d.rows; r += 1024) {
+  for (int64_t r = first; r < d.rows; r += step) {
     const int t = d.label[r];
     const float w = d.weight ? d.weight[r] : 1.f;
     loss += (double)d.value[r];
     total += t >= 0 && t < d.V ? (double)w : 0.0;
+  }
+}
+
+__global__ void __launch_bounds__(1024) policy_parts_kernel(TokenLossDesc d) {
+  double loss = 0.0, total = 0.0;
+  add_rows(d, (int64_t)blockIdx.x * 1024 + threadIdx.x, 1024 * kParts, loss,
+           total);
+  block_sums(loss, total);
+  if (threadIdx.x == 0) {
+    d.sums[2 * blockIdx.x] = loss;
+    d.sums[2 * blockIdx.x + 1] = total;
+  }
+}
+
+__global__ void __launch_bounds__(1024)
+    policy_total_kernel(TokenLossDesc d, bool parts) {
+  double loss = 0.0, total = 0.0;
+  if (!parts) {
+    add_rows(d, threadIdx.x, 1024, loss, total);
+  } else if (threadIdx.x < kParts) {
+    loss = d.sums[2 * threadIdx.x];
+    total = d.sums[2 * threadIdx.x + 1];
   }
   block_sums(loss, total);
   if (threadIdx.x != 0) return;
@@ -281,8 +309,19 @@ __global__ void __launch_bounds__(1024) policy_total_kernel(TokenLossDesc d) {
   d.total[0] = (float)(1.0 / total);
 }
 
+// sum of a sequence's values, a workgroup for each
 __global__ void __launch_bounds__(1024)
-    preference_total_kernel(TokenLossDesc d) {
+    preference_parts_kernel(TokenLossDesc d) {
+  const float *v = d.value + (int64_t)blockIdx.x * d.seq;
+  double sum = 0.0, none = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < d.seq; i += 1024) sum += (double)v[i];
+  block_sums(sum, none);
+  if (threadIdx.x == 0) d.sums[blockIdx.x] = sum;
+}
+
+__global__ void __launch_bounds__(1024)
+    preference_total_kernel(TokenLossDesc d, bool parts) {
   __shared__ double share[16];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t seqs = 2 * d.pairs;
@@ -290,7 +329,7 @@ __global__ void __launch_bounds__(1024)
   int each = 1;
   while (each < 16 && 2 * each * seqs <= 16) each <<= 1;
   const int at_once = 16 / each, mine = wave / each, sub = wave % each;
-  for (int64_t first = 0; first < seqs; first += at_once) {
+  for (int64_t first = 0; !parts && first < seqs; first += at_once) {
     const int64_t q = first + mine;
     double sum = 0.0;
     if (q < seqs) {
@@ -303,10 +342,10 @@ __global__ void __launch_bounds__(1024)
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
     if (lane == 0) share[wave] = sum;
     __syncthreads();
-    if (threadIdx.x < at_once && first + threadIdx.x < seqs) {
+    if ((int)threadIdx.x < at_once && first + threadIdx.x < seqs) {
       double a = 0.0;
       for (int k = 0; k < each; ++k) a += share[threadIdx.x * each + k];
-      d.seq_sum[first + threadIdx.x] = a;
+      d.sums[first + threadIdx.x] = a;
     }
     __syncthreads();
   }
@@ -315,7 +354,7 @@ __global__ void __launch_bounds__(1024)
   double loss = 0.0, none = 0.0;
   const double smooth = d.smoothing, beta = d.beta;
   for (int64_t i = threadIdx.x; i < d.pairs; i += 1024) {
-    const double z = beta * (d.seq_sum[i] - d.seq_sum[d.pairs + i]);
+    const double z = beta * (d.sums[i] - d.sums[d.pairs + i]);
     loss += (1.0 - smooth) * soft_plus(-z) + smooth * soft_plus(z);
     const double up = 1.0 / (1.0 + exp(-z)), down = 1.0 / (1.0 + exp(z));
     d.total[i] = (float)((smooth * up - (1.0 - smooth) * down) * beta /
@@ -333,8 +372,9 @@ __global__ void __launch_bounds__(1024)
 template <typename T, int VEC, int WPR, bool STREAM>
 __global__ void __launch_bounds__(threads_of(WPR))
     token_grad_kernel(TokenLossDesc d) {
-  const int64_t q =
-      WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int64_t q = d.first + (WPR == 1 ? (int64_t)blockIdx.x * 4 +
+                                              (threadIdx.x >> 6)
+                                        : blockIdx.x);
   if (q >= d.rows) return;
   const int64_t r = d.rows - 1 - q;
   const int tid = threadIdx.x & (64 * WPR - 1), threads = 64 * WPR;
@@ -423,30 +463,35 @@ constexpr int64_t kLongRow = 32 << 10;
 // (8192 x 50257 bf16: 356 us instead of 388, 4096 x 30522 114 instead of 134).
 constexpr int64_t kStreamBytes = 128 << 20;
 
+// rows of one launch: its threads are counted in 32 bits
+constexpr int64_t kLaunchRows = 1 << 22;
+
 template <typename T, int VEC>
-void launch_rows(const TokenLossDesc &d, int pieces, hipStream_t s) {
+void launch_rows(const TokenLossDesc &d, int64_t rows, int pieces,
+                 hipStream_t s) {
   if (d.V <= kWaveRow)
     hipLaunchKernelGGL((token_rows_kernel<T, VEC, 1>),
-                       dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, s, d);
+                       dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, d);
   else if (d.piece * (int64_t)sizeof(T) < kLongRow)
     hipLaunchKernelGGL((token_rows_kernel<T, VEC, 4>),
-                       dim3((unsigned)d.rows, pieces), dim3(256), 0, s, d);
+                       dim3((unsigned)rows, pieces), dim3(256), 0, s, d);
   else
     hipLaunchKernelGGL((token_rows_kernel<T, VEC, 8>),
-                       dim3((unsigned)d.rows, pieces), dim3(512), 0, s, d);
+                       dim3((unsigned)rows, pieces), dim3(512), 0, s, d);
 }
 
 template <typename T, int VEC, bool STREAM>
-void launch_grad(const TokenLossDesc &d, int pieces, hipStream_t s) {
+void launch_grad(const TokenLossDesc &d, int64_t rows, int pieces,
+                 hipStream_t s) {
   if (d.V <= kWaveRow)
     hipLaunchKernelGGL((token_grad_kernel<T, VEC, 1, STREAM>),
-                       dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, s, d);
+                       dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, d);
   else if (d.piece * (int64_t)sizeof(T) < kLongRow)
     hipLaunchKernelGGL((token_grad_kernel<T, VEC, 4, STREAM>),
-                       dim3((unsigned)d.rows, pieces), dim3(256), 0, s, d);
+                       dim3((unsigned)rows, pieces), dim3(256), 0, s, d);
   else
     hipLaunchKernelGGL((token_grad_kernel<T, VEC, 8, STREAM>),
-                       dim3((unsigned)d.rows, pieces), dim3(512), 0, s, d);
+                       dim3((unsigned)rows, pieces), dim3(512), 0, s, d);
 }
 
 // whether every row of a and b has its 16-byte boundaries at the same places
@@ -471,6 +516,12 @@ int sa_token_loss_pieces(int64_t rows, int64_t V) {
   return p < 1 ? 1 : (int)p;
 }
 
+// float64 words of `sums` that a loss needs
+int64_t sa_token_loss_sums(int mode, int64_t rows, int64_t pairs) {
+  if (mode == kPreference) return 2 * pairs;
+  return mode == kPolicy && rows > kOneBlockRows ? 2 * kParts : 0;
+}
+
 static int64_t piece_of(int64_t V, int pieces) {
   return ((V + pieces - 1) / pieces + 63) / 64 * 64;
 }
@@ -480,36 +531,52 @@ int sa_token_loss_fwd(int dtype, const TokenLossDesc *desc, hipStream_t s) {
   if (int rc = check_desc(d)) return rc;
   const int pieces = sa_token_loss_pieces(d.rows, d.V);
   d.piece = piece_of(d.V, pieces);
-  if (pieces > 1 && !d.part) return -2;
-  if (d.rows > 0) {
-    SA_DISPATCH_FLOAT(dtype, T, {
-      launch_rows<T, 16 / (int)sizeof(T)>(d, pieces, s);
-      if (pieces > 1)
-        hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)d.rows),
-                           dim3(64), 0, s, d, pieces);
-    });
+  const bool parts = d.rows > kOneBlockRows;
+  if ((pieces > 1 && !d.part) ||
+      (sa_token_loss_sums(d.mode, d.rows, d.pairs) > 0 && !d.sums))
+    return -2;
+  SA_DISPATCH_FLOAT(dtype, T, {
+    for (d.first = 0; d.first < d.rows; d.first += kLaunchRows)
+      launch_rows<T, 16 / (int)sizeof(T)>(d, i64min(kLaunchRows, d.rows - d.first),
+                                          pieces, s);
+    if (pieces > 1)
+      hipLaunchKernelGGL((token_join_kernel<T>), dim3((unsigned)d.rows),
+                         dim3(64), 0, s, d, pieces);
+  });
+  if (d.mode == kPolicy) {
+    if (parts)
+      hipLaunchKernelGGL(policy_parts_kernel, dim3(kParts), dim3(1024), 0, s, d);
+    hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, s, d, parts);
+  } else if (d.mode == kPreference && d.pairs > 0) {
+    // (a workgroup for each of up to 2^21 sequences: threads in 32 bits)
+    const bool many = parts && d.pairs <= (1 << 20);
+    if (many)
+      hipLaunchKernelGGL(preference_parts_kernel, dim3((unsigned)(2 * d.pairs)),
+                         dim3(1024), 0, s, d);
+    hipLaunchKernelGGL(preference_total_kernel, dim3(1), dim3(1024), 0, s, d,
+                       many);
   }
-  if (d.mode == kPolicy)
-    hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(1024), 0, s, d);
-  else if (d.mode == kPreference && d.pairs > 0)
-    hipLaunchKernelGGL(preference_total_kernel, dim3(1), dim3(1024), 0, s, d);
   return 0;
 }
 
 int sa_token_loss_bwd(int dtype, const TokenLossDesc *desc, hipStream_t s) {
   TokenLossDesc d = *desc;
   if (int rc = check_desc(d)) return rc;
-  if (d.rows == 0) return 0;
   const int pieces = sa_token_loss_pieces(d.rows, d.V);
   d.piece = piece_of(d.V, pieces);
   const bool wide = same_phase(d.x, d.dx);
   SA_DISPATCH_FLOAT(dtype, T, {
-    if (!wide)
-      launch_grad<T, 1, false>(d, pieces, s);
-    else if (d.rows * d.V * (int64_t)sizeof(T) > kStreamBytes)
-      launch_grad<T, 16 / (int)sizeof(T), true>(d, pieces, s);
-    else
-      launch_grad<T, 16 / (int)sizeof(T), false>(d, pieces, s);
+    const bool stream = d.rows * d.V * (int64_t)sizeof(T) > kStreamBytes;
+    constexpr int kVec = 16 / (int)sizeof(T);
+    for (d.first = 0; d.first < d.rows; d.first += kLaunchRows) {
+      const int64_t rows = i64min(kLaunchRows, d.rows - d.first);
+      if (!wide)
+        launch_grad<T, 1, false>(d, rows, pieces, s);
+      else if (stream)
+        launch_grad<T, kVec, true>(d, rows, pieces, s);
+      else
+        launch_grad<T, kVec, false>(d, rows, pieces, s);
+    }
   });
   return 0;
 }

@@ -1240,6 +1240,47 @@ def test_operands_of_another_device_are_refused(gpu_dev, cpu_dev):
 
 
 @pytest.mark.gpu
+def test_many_rows(gpu_dev):
+    """More rows than one launch takes, and sums over more than one workgroup
+    adds up."""
+    N, V = (1 << 22) + 5, 3
+    x, t = logits(1, "float16", N, V), labels(2, V, N)
+    x[-5:], t[-5:] = x[:5], torch.tensor([0, 1, 2, -1, 1])
+    lp, used = log_prob64(x, t)
+    old = rounded(lp + 0.1 * normal(3, N), "float32")
+    adv = rounded(normal(4, N), "float32")
+    tx, tt = put(gpu_dev, x, "float16"), put(gpu_dev, t)
+    op = autograd.TokenLogProb(tt)
+    check(op(tx)[0], lp, scale=rows_room(V) + 64 * E32)
+    check_dx(op.backward(put(gpu_dev, adv).data), adv, x, t, used, "float16",
+             4 * E32)
+    op = autograd.PolicyLoss(tt, put(gpu_dev, old), put(gpu_dev, adv))
+    want, g = loss_and_coefficients(
+        lambda v: policy64(v, t, old, adv, None, None, (0.2, 0.2), 0.0), x, t)
+    # each token's term good to a few roundings of at most |r A|
+    check(op(tx)[0], want.reshape(1), scale=float((4 * adv.abs()).mean()) *
+          (rows_room(V) + 32 * E32))
+    dx = got(op.backward(float(N))).view(N, V)
+    room = HALF["float16"] * (N * g).abs() + 2.0 ** -25 + \
+        4 * adv.abs().unsqueeze(-1) * 64 * (rows_room(V) + 32 * E32)
+    assert ((dx - N * g).abs() <= room).all()
+    # 2 x 2100 sequences of 9: a workgroup for each
+    P, S = 2100, 9
+    x, t = x[:2 * P * S].view(2 * P, S, V), t[:2 * P * S].view(2 * P, S)
+    ref = rounded(lp[:2 * P * S].view(2 * P, S) + 0.3 * normal(5, 2 * P, S),
+                  "float32")
+    op = autograd.PreferenceLoss(put(gpu_dev, t), put(gpu_dev, ref), 0.5, 0.1)
+    y = op(put(gpu_dev, x, "float16"))[0]
+    want, g = loss_and_coefficients(
+        lambda v: preference64(v, t, ref, 0.5, 0.1), x, t)
+    off = 0.5 * 2 * S * (rows_room(V) + 16 * E32)
+    check(y, want.reshape(1), scale=off + 8 * E32)
+    dx = got(op.backward(float(P))).view(2 * P, S, V)
+    assert ((dx - P * g).abs() <= HALF["float16"] * (P * g).abs() +
+            2.0 ** -25 + 0.5 * (rows_room(V) + 2 * off + 32 * E32)).all()
+
+
+@pytest.mark.gpu
 def test_results_repeat(gpu_dev):
     """No atomics: the same call gives the same bits."""
     handle = singa_wrap.RotaryHandle(128)
