@@ -93,13 +93,25 @@ __device__ __forceinline__ void advance(const Consts &c, float g, float &p,
   p = p - c.lr * ((m * c.c1) / (sqrtf(v * c.c2) + c.eps));
 }
 
+// The square root rounded to nearest: the hardware's, good to one unit in the
+// last place, or the neighbour whose product with it says so.  (A v below
+// 2^-126 may count as 0: its root, 2^-63 at most, is nothing beside eps.)
+__device__ __forceinline__ float root(float v) {
+  const float s = __builtin_amdgcn_sqrtf(v);
+  const float down = __uint_as_float(__float_as_uint(s) - 1u);
+  const float up = __uint_as_float(__float_as_uint(s) + 1u);
+  const float too_large = fmaf(-down, s, v), too_small = fmaf(-up, s, v);
+  float r = too_large <= 0.f ? down : s;
+  return too_small > 0.f ? up : r;
+}
+
 // The same with r = sqrt(v) in the place of v.  The step takes the root that
 // the state needs anyway, and a reciprocal good to one unit in the last place.
 __device__ __forceinline__ void advance8(const Consts &c, float g, float &p,
                                          float &m, float &r) {
   g = g * c.scale;
   m = c.b1 * m + c.k1 * g;
-  r = sqrtf(c.b2 * (r * r) + c.k2 * (g * g));
+  r = root(c.b2 * (r * r) + c.k2 * (g * g));
   const float u =
       (m * c.c1) * __builtin_amdgcn_rcpf(fmaf(r, c.root_c2, c.eps));
   p = fmaf(-c.decay, p, p);
@@ -254,59 +266,88 @@ __device__ __forceinline__ Words philox(uint32_t c0, uint32_t c1, uint32_t c2,
   return {{c0, c1, c2, c3}};
 }
 
+// Magnitudes are compared as integers: the bits of non-negative floats are in
+// their order, infinity and NaN above all numbers, and no instruction is spent
+// on quieting NaN.
+constexpr uint32_t kInfinity = 0x7f800000u;
+
+__device__ __forceinline__ uint32_t magnitude(float x) {
+  return __float_as_uint(x) & 0x7fffffffu;
+}
+
+// the larger of x and of what the lane pattern brings (0 where nothing)
 template <int CTRL, int ROWS>
-__device__ __forceinline__ float max_dpp(float x) {
-  const int other = __builtin_amdgcn_update_dpp(
-      __float_as_int(x), __float_as_int(x), CTRL, ROWS, 0xf, false);
-  return fmaxf(x, __int_as_float(other));
+__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+  const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(
+      0, (int)x, CTRL, ROWS, 0xf, ROWS == 0xf);
+  return x > other ? x : other;
 }
 
 // The largest of a wave's values, in a scalar register: within rows of 16 lanes
 // (neighbours, pairs, half rows, rows), then into the following rows.
-__device__ __forceinline__ float wave_top(float x) {
+__device__ __forceinline__ uint32_t wave_top(uint32_t x) {
   x = max_dpp<0xb1, 0xf>(x);    // quad_perm 1 0 3 2
   x = max_dpp<0x4e, 0xf>(x);    // quad_perm 2 3 0 1
   x = max_dpp<0x141, 0xf>(x);   // row_half_mirror
   x = max_dpp<0x140, 0xf>(x);   // row_mirror
   x = max_dpp<0x142, 0xa>(x);   // row_bcast15 into rows 1 and 3
   x = max_dpp<0x143, 0xc>(x);   // row_bcast31 into rows 2 and 3
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// The largest finite magnitude of the wave's 256 values (NaN loses every
-// comparison of fmaxf; infinities are looked for only where there is one).
-__device__ __forceinline__ float block_top(const float *x) {
-  float top = wave_top(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
-                             fmaxf(fabsf(x[2]), fabsf(x[3]))));
-  if (top == INFINITY) {
-    top = 0.f;
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) {
+  return a > b ? a : b;
+}
+
+// The largest finite magnitude of the wave's 256 values; `finite`: whether all
+// are (what is not is looked for only where there is some).
+__device__ __forceinline__ float block_top(const float *x, bool &finite) {
+  uint32_t top = wave_top(umax(umax(magnitude(x[0]), magnitude(x[1])),
+                               umax(magnitude(x[2]), magnitude(x[3]))));
+  finite = top < kInfinity;
+  if (!finite) {
+    top = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float a = fabsf(x[j]);
-      top = fmaxf(top, a < INFINITY ? a : 0.f);
+      const uint32_t a = magnitude(x[j]);
+      top = umax(top, a < kInfinity ? a : 0u);
     }
     top = wave_top(top);
   }
   // below this the reciprocal of the scale would overflow: zeros
-  return top > 0x1p-110f ? top : 0.f;
+  return __uint_as_float(top > 0x08800000u ? top : 0u);   // 2^-110
 }
 
 // x times inv, rounded to e4m3 by the 16 bits of noise: floor(s / unit + u) of
 // the codes' spacing.  A normal code keeps three bits of the fraction: the
 // noise is added behind them, a carry goes where it should, the rest is cut
-// off.  Below 2^-6 the spacing is 2^-9 throughout.
-template <bool KEEP>
+// off.  Below 2^-6 the spacing is 2^-9 throughout.  ROOT: x is not negative,
+// and what is positive does not become zero.  FINITE: so are all values.
+template <bool ROOT, bool FINITE>
 __device__ __forceinline__ float to_code(float x, float inv, uint32_t noise) {
-  const float s = x * inv, size = fabsf(s);
-  const float normal =
-      __uint_as_float((__float_as_uint(size) + (noise << 4)) & 0xfff00000u);
-  const float small =
-      floorf(size * 512.f + (float)noise * 0x1p-16f) * 0x1p-9f;
-  float q = size < 0x1p-6f ? small : normal;
-  if (KEEP) q = size > 0.f ? fmaxf(q, 0x1p-9f) : q;
-  q = q > 448.f ? 448.f : q;
-  q = size < INFINITY ? q : NAN;
-  return copysignf(q, s);
+  const float s = x * inv;
+  const uint32_t size = magnitude(s);
+  const uint32_t normal = (size + (noise << 4)) & 0xfff00000u;
+  float small = floorf(fmaf((float)noise, 0x1p-16f,
+                            __uint_as_float(size) * 512.f)) * 0x1p-9f;
+  if (ROOT)
+    small = size > 0 ? __uint_as_float(umax(__float_as_uint(small), 0x3b000000u))
+                     : small;   // 2^-9
+  uint32_t q = size < 0x3c800000u ? __float_as_uint(small) : normal;   // 2^-6
+  q = q < 0x43e00000u ? q : 0x43e00000u;   // 448
+  if (!FINITE) q = size < kInfinity ? q : 0x7fc00000u;
+  const float f = __uint_as_float(q);
+  return ROOT ? f : copysignf(f, s);
+}
+
+template <bool FINITE>
+__device__ __forceinline__ void to_codes(float *m, float *r, float mi, float ri,
+                                         const uint32_t *words) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    m[j] = to_code<false, FINITE>(m[j], mi, words[j] & 0xffffu);
+    r[j] = to_code<true, FINITE>(r[j], ri, words[j] >> 16);
+  }
 }
 
 __device__ __forceinline__ uint32_t pack_codes(const float *q) {
@@ -360,17 +401,17 @@ __device__ __forceinline__ void chunk8(const Consts &c, T *p16, P *p,
       advance8(c, gf[k][j], pf[k][j], m[j], v[j]);
     store4<A, P>(p + i, pf[k], n, wide);
     if (MASTER) store4<A, T>(p16 + i, pf[k], n, wide);
-    const float mt = block_top(m), rt = block_top(v);
+    bool m_finite, r_finite;
+    const float mt = block_top(m, m_finite), rt = block_top(v, r_finite);
     const float mi = mt > 0.f ? 448.f * (1.f / mt) : 0.f;
     const float ri = rt > 0.f ? 448.f * (1.f / rt) : 0.f;
     const int64_t group = (base + i) / 4;
     const Words u = philox((uint32_t)group, (uint32_t)((uint64_t)group >> 32),
                            step, 0u, seed);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[j] = to_code<false>(m[j], mi, u.w[j] & 0xffffu);
-      v[j] = to_code<true>(v[j], ri, u.w[j] >> 16);
-    }
+    if (m_finite && r_finite)   // the same for the whole wave
+      to_codes<true>(m, v, mi, ri, u.w);
+    else
+      to_codes<false>(m, v, mi, ri, u.w);
     store_word<A>(mw + i / 4, pack_codes(m));
     store_word<A>(rw + i / 4, pack_codes(v));
     if (lane == 0) {
