@@ -21,9 +21,15 @@
 //  * The step itself uses the moments before they are rounded.
 //
 // Bound by memory: float32 reads p, g, m, v and writes p, m, v, 28 bytes an
-// element; bfloat16 with masters and 8-bit states 16 bytes.  Compiled without
-// contraction, so that a state is the same value a plain evaluation of the
-// formula in float32 gives.
+// element; bfloat16 with masters and 8-bit states moves 16.  A workgroup of 256
+// has 4096 elements in registers, all their loads issued before the first is
+// used; a whole chunk of them is accessed without bounds.  141 M parameters:
+// float32 680 us (5.8 TB/s), bfloat16 with masters 726 us (5.5 TB/s), 8-bit
+// states 397 us with float32 and 400 us with bfloat16 parameters (5.7 TB/s),
+// where a large copy reaches 5.1 TB/s.  The 8-bit kernel issues some 400
+// instructions for each four elements of a lane: the rate of the vector units is
+// not far behind the memory's.  Compiled without contraction, so that a state is
+// the same value a plain evaluation of the formula in float32 gives.
 //
 // The reference has Adam only (python/singa/opt.py:608-683), one element-wise
 // launch for each operation.
