@@ -20,16 +20,17 @@
 //    NaN: it spoils its own element, as a float32 state would, not 255 others.
 //  * The step itself uses the moments before they are rounded.
 //
-// Bound by memory: float32 reads p, g, m, v and writes p, m, v, 28 bytes an
-// element; bfloat16 with masters and 8-bit states moves 16.  A workgroup of 256
-// has 4096 elements in registers, all their loads issued before the first is
-// used; a whole chunk of them is accessed without bounds.  141 M parameters:
+// float32 states are bound by memory: p, g, m, v are read and p, m, v written, 28
+// bytes an element; bfloat16 with masters and 8-bit states moves 16.  A workgroup
+// of 256 has 4096 elements in registers, all their loads issued before the first
+// is used; a whole chunk of them is accessed without bounds.  141 M parameters:
 // float32 680 us (5.8 TB/s), bfloat16 with masters 726 us (5.5 TB/s), 8-bit
 // states 397 us with float32 and 400 us with bfloat16 parameters (5.7 TB/s),
-// where a large copy reaches 5.1 TB/s.  The 8-bit kernel issues some 400
-// instructions for each four elements of a lane: the rate of the vector units is
-// not far behind the memory's.  Compiled without contraction, so that a state is
-// the same value a plain evaluation of the formula in float32 gives.
+// where a large copy reaches 5.1 TB/s.  The 8-bit kernel issues some 390
+// instructions for each four elements of a lane, which keeps the vector units
+// busy throughout: they bound it, not the memory.  Compiled without contraction,
+// so that a state is the same value a plain evaluation of the formula in float32
+// gives.
 //
 // The reference has Adam only (python/singa/opt.py:608-683), one element-wise
 // launch for each operation.

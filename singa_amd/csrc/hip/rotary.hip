@@ -24,7 +24,7 @@
 // sin of a token are computed once by the workgroup into LDS and shared by its
 // heads.  The frequencies travel in the kernel arguments, so a handle owns no
 // device memory.  2 x 4096 tokens of 32 + 8 heads of 128, bfloat16, normed:
-// forward 33 us, backward 50 us (5.0 TB/s each; a large copy reaches 5.1), and
+// forward 34 us, backward 50 us (4.9 and 5.0 TB/s; a large copy reaches 5.1), and
 // 4 us to add up the scale gradients; one token for each of 16 sequences 4.5 us.
 //
 // The reference has no such operator.

@@ -19,7 +19,7 @@
 // on every row -- and writes the gradient; the probabilities never reach
 // memory.  Maxima, sums and log-probabilities are float32, sums over tokens
 // float64.  8192 x 50257 bfloat16 logits, three tenths of the tokens ignored:
-// forward 102 us (5.6 TB/s of what is read), backward 255 us (5.5 TB/s); a large
+// forward 102 us (5.6 TB/s of what is read), backward 252 us (5.5 TB/s); a large
 // copy reaches 5.1 TB/s.  Few rows are cut into pieces (8 x 131071 float32: 4 us
 // and 3.5 us to join them).
 //
