@@ -124,6 +124,12 @@ class RotaryHandle(object):
         self.turns_address = self._turns.ctypes.data
         self.half = layout == "half"
 
+    def __setstate__(self, state):
+        # a copy has a table of its own: the original's may be gone
+        self.__dict__.update(state)
+        self._turns = self._turns.copy()
+        self.turns_address = self._turns.ctypes.data
+
 
 def _described(t):
     return "%s %s" % (tuple(t._shape), dtypes.name(t._dtype))

@@ -4,7 +4,11 @@ AdamW against plain float64 evaluations, on the host and on the MI355X.
 Tolerances count roundings: half a step of the result's type, relative to it
 (fp32 2^-24, fp16 2^-11, bf16 2^-8), plus a number of float32 roundings of the
 intermediate values, each at most 2^-24 of the values' scale."""
+import copy
+import gc
 import math
+import pickle
+import weakref
 
 import numpy as np
 import pytest
@@ -1307,3 +1311,14 @@ def test_devices_agree_on_the_handle(cpu_dev):
     turns = h._turns.astype(np.float64) / 2.0 ** 64
     np.testing.assert_allclose(turns * 2 * np.pi, h.frequencies, rtol=1e-14)
     assert device.get_default_device() is cpu_dev
+
+
+def test_handle_copies_own_their_turns(cpu_dev):
+    """A copied or unpickled handle addresses its own table."""
+    h = singa_wrap.RotaryHandle(64, 32, layout="interleaved",
+                                scaling=("linear", 4.0))
+    for other in (copy.copy(h), copy.deepcopy(h),
+                  pickle.loads(pickle.dumps(h))):
+        assert other.turns_address == other._turns.ctypes.data
+        assert (other._turns == h._turns).all()
+        assert (other.half, other.rotary_dim) == (h.half, h.rotary_dim)
