@@ -22,6 +22,7 @@ DistOpt :686-1094).
 """
 import itertools
 import operator
+import weakref
 from collections import OrderedDict
 
 from . import autograd
@@ -593,7 +594,7 @@ class AdamW(Optimizer):
             tables.append(self.masters)
         found = self._groups.get(at)
         if found is not None:
-            group, kept, keys, columns = found
+            group, _, keys, columns = found
             if not (_same(group.params, list(map(_core, params))) and
                     all([_same(column, list(map(table.get, keys)))
                          for table, column in zip(tables, columns)]) and
@@ -605,8 +606,13 @@ class AdamW(Optimizer):
             group = singa.AdamWGroup(list(map(_core, params)),
                                      [list(map(_core, c)) for c in columns],
                                      mixed)
-            # the parameters are kept with it: an id is theirs while they live
-            self._groups[at] = (group, params, keys, columns)
+            # A group keeps its parameters' memory: those of which a parameter is
+            # gone are dropped.  (Its core tensors tell a new parameter under
+            # the id of an old one.)
+            self._groups = {k: kept for k, kept in self._groups.items()
+                            if all([r() is not None for r in kept[1]])}
+            self._groups[at] = (group, list(map(weakref.ref, params)), keys,
+                                columns)
         singa.AdamWUpdateMulti(group, list(map(_core, grads)), hypers,
                                self.state_bits, scale, self.seed)
 

@@ -1322,3 +1322,29 @@ def test_handle_copies_own_their_turns(cpu_dev):
         assert other.turns_address == other._turns.ctypes.data
         assert (other._turns == h._turns).all()
         assert (other.half, other.rotary_dim) == (h.half, h.rotary_dim)
+
+
+def test_adamw_lets_go_of_replaced_parameters(dev):
+    """What a step kept of a parameter that is gone is dropped by the next
+    step that looks states up; one that lives keeps its own."""
+    o = opt.AdamW(lr=0.1)
+    stays = put(dev, normal(1, 40))
+    o.apply_many([(stays, put(dev, normal(2, 40)))])
+    gone = []
+    for _ in range(4):
+        p = put(dev, normal(1, 300))
+        p.name = "w"
+        o.apply_many([(p, put(dev, normal(2, 300)))])
+        gone.append(weakref.ref(p.data))
+        del p
+        gc.collect()
+    # the last one stays until something else is looked up
+    assert [r() is None for r in gone] == [True] * 3 + [False]
+    q = put(dev, normal(1, 20))
+    o.apply_many([(q, put(dev, normal(2, 20)))])
+    gc.collect()
+    assert gone[-1]() is None and len(o._groups) == 2
+    # both of those live: the same group is found again
+    found = dict(o._groups)
+    o.apply_many([(stays, put(dev, normal(2, 40)))])
+    assert all(o._groups[k] is v for k, v in found.items())
