@@ -490,6 +490,8 @@ class CpuMath(object):
         k1, k2, decay = float(one - b1), float(one - b2), float(lr * wd)
         lr, eps, b1, b2 = float(lr), float(eps), float(b1), float(b2)
         for i, n in enumerate(sizes):
+            if n == 0:
+                continue
             p = masters[i] if masters else ps[i]
             g = gs[i][:n].float() * scale
             if state_bits == 32:

@@ -1348,3 +1348,25 @@ def test_adamw_lets_go_of_replaced_parameters(dev):
     found = dict(o._groups)
     o.apply_many([(stays, put(dev, normal(2, 40)))])
     assert all(o._groups[k] is v for k, v in found.items())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_empty_parameters(dev, bits):
+    """Parameters of no elements among others are stepped over."""
+    for order in ((0, 700), (700, 0), (0, 0, 700, 0, 5), (0,)):
+        o = opt.AdamW(lr=0.1, state_bits=bits)
+        alone = opt.AdamW(lr=0.1, state_bits=bits)
+        a, b = [], []
+        for i, n in enumerate(order):
+            g = put(dev, normal(10 + i, n))
+            p, q = put(dev, normal(i, n)), put(dev, normal(i, n))
+            a.append((p, g))
+            if n:
+                b.append((q, g))
+        for _ in range(2):
+            o.apply_many(a)
+            alone.apply_many(b)
+            o.step()
+            alone.step()
+        for (p, _), (q, _) in zip([e for e in a if e[0].size()], b):
+            assert (got(p) == got(q)).all()
