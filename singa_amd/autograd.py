@@ -1314,8 +1314,8 @@ class PolicyLoss(_TokenLoss):
         loss = sum w (-min(r A, clip(r, 1 - clip[0], 1 + clip[1]) A)
                       + kl (exp(d) - d - 1)) / sum w
 
-    old (the sampling policy's log-probabilities), advantages, weights (1
-    without; a token of weight 0 takes no part) and reference (no divergence
+    old (the sampling policy's log-probabilities), advantages, weights (from 0,
+    1 without; a token of weight 0 takes no part) and reference (no divergence
     term without) have the labels' shape.  0 when the weights that take part
     add up to 0."""
     takes_scalar_dy = True

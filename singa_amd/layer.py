@@ -793,15 +793,16 @@ class RotaryQK(Layer):
     ``singa_wrap.RotaryHandle``."""
 
     def __init__(self, rotary_dim=None, base=10000.0, layout="half",
-                 scaling=None, norm=False, eps=1e-6):
+                 scaling=None, norm=False, eps=1e-6, amplitude=None):
         super().__init__()
         _keep(self, locals(), 'rotary_dim', 'base', 'layout', 'scaling',
-              'norm', 'eps')
+              'norm', 'eps', 'amplitude')
 
     def initialize(self, q, k, positions=None):
         d = q.shape[-1]
         self.handle = singa.RotaryHandle(d, self.rotary_dim, self.base,
-                                         self.layout, self.scaling)
+                                         self.layout, self.scaling,
+                                         self.amplitude)
         if self.norm:
             self._new_param('q_scale', (d,), q, _constant(1.0), q.dtype)
             self._new_param('k_scale', (d,), q, _constant(1.0), q.dtype)

@@ -1370,3 +1370,12 @@ def test_adamw_empty_parameters(dev, bits):
             alone.step()
         for (p, _), (q, _) in zip([e for e in a if e[0].size()], b):
             assert (got(p) == got(q)).all()
+
+
+def test_rotary_layer_amplitude(dev):
+    """The layer takes the handle's amplitude."""
+    q, k = (put(dev, normal(s, 1, 3, 2, 8)) for s in (1, 2))
+    plain = layer.RotaryQK()(q, k)
+    twice = layer.RotaryQK(amplitude=2.0)(q, k)
+    for a, b in zip(plain, twice):
+        assert (got(b) == 2.0 * got(a)).all()
