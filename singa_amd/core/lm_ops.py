@@ -13,6 +13,7 @@ import operator
 import numpy as np
 
 from . import dtypes
+from .. import _rt
 from .tensor_core import Contiguous, Tensor, _one_device, _submit
 
 _FLOATS = (dtypes.kFloat32, dtypes.kFloat16, dtypes.kBFloat16)
@@ -337,7 +338,6 @@ class TokenLoss(object):
 ADAMW_BLOCK = 256       # values that share the scale of an 8-bit state
 
 
-_stored = operator.attrgetter("_block.data")
 _typed = operator.attrgetter("_dtype")
 _held_in = operator.attrgetter("_block")
 _placed = operator.attrgetter("_dev")
@@ -350,7 +350,8 @@ class AdamWGroup(object):
     moment and of the root of the second, in whole blocks of 256 values, and a
     float32 scale for each block; behind them, when ``mixed``, the float32
     master copies of 16-bit parameters.  It holds while every tensor in it
-    keeps its storage (``storage``: parameters, then each list of states)."""
+    keeps its block and storage (``holding``: parameters, then each list of
+    states)."""
 
     def __init__(self, params, states, mixed):
         self.params, self.states = params, states
@@ -364,9 +365,9 @@ class AdamWGroup(object):
         _one_device("AdamWUpdateMulti", self.dev, self.members)
         self.sizes = [p.Size() for p in params]
         self.strides = [p._stride for p in params]
-        self.storage = [t._storage() for t in self.members]
-        self.columns = [self.storage[i:i + n]
-                        for i in range(0, len(self.storage), n)]
+        storage = [t._storage() for t in self.members]
+        self.columns = [storage[i:i + n] for i in range(0, len(storage), n)]
+        self.holding = _rt.Holding(list(map(_held_in, self.members)))
         self.addresses = [[t.data_ptr() for t in c] for c in self.columns]
 
 
@@ -383,10 +384,12 @@ def AdamWUpdateMulti(group, grads, hypers, state_bits=32, scale=1.0, seed=0):
         _one_device("AdamWUpdateMulti", dev, [*grads, *hypers])
     scale, seed, state_bits = float(scale), int(seed), int(state_bits)
     if not dev.graph_enabled():
-        flat = [t._storage() for t in hypers]
+        flat = _rt.storages(list(map(_held_in, itertools.chain(grads, hypers))))
+        if any(map(operator.is_, flat, itertools.repeat(None))):
+            flat = [t._storage() for t in itertools.chain(grads, hypers)]
         dev.math.adamw_update_multi(
-            group.sizes, group.columns, [g._storage() for g in grads],
-            group.mixed, flat, state_bits, scale, seed, group.addresses)
+            group.sizes, group.columns, flat[:n], group.mixed, flat[n:],
+            state_bits, scale, seed, group.addresses)
         return
     sizes, mixed = group.sizes, group.mixed
 

@@ -33,9 +33,36 @@ class PyBlock : public Block {
   void free_data() override { data_ = py::none(); }
   py::object get() const { return data_; }
   void set(py::object o) { data_ = std::move(o); }
+  bool holds(const py::object &o) const { return data_.is(o); }
 
  private:
   py::object data_;
+};
+
+// Blocks and the storage each of them has now.
+class Holding {
+ public:
+  explicit Holding(const py::list &blocks) {
+    for (const py::handle b : blocks) {
+      // the Python objects keep their blocks alive
+      objects_.push_back(py::reinterpret_borrow<py::object>(b));
+      blocks_.push_back(&b.cast<PyBlock &>());
+      storage_.push_back(blocks_.back()->get());
+    }
+  }
+  // whether `blocks` are these, and each still has its storage
+  bool Same(const py::list &blocks) const {
+    if (blocks.size() != objects_.size()) return false;
+    for (size_t i = 0; i < objects_.size(); ++i)
+      if (PyList_GET_ITEM(blocks.ptr(), (Py_ssize_t)i) != objects_[i].ptr() ||
+          !blocks_[i]->holds(storage_[i]))
+        return false;
+    return true;
+  }
+
+ private:
+  std::vector<py::object> objects_, storage_;
+  std::vector<PyBlock *> blocks_;
 };
 
 BlockVec ToBlocks(const std::vector<std::shared_ptr<PyBlock>> &v) {
@@ -85,6 +112,21 @@ PYBIND11_MODULE(_rt, m) {
       .def("IncRefCount", &PyBlock::IncRefCount)
       .def("DecRefCount", &PyBlock::DecRefCount)
       .def("ref_count", &PyBlock::ref_count);
+
+  // An optimizer's step looks at the blocks of all its tensors: in one call each,
+  // whether they and their storage are those of an earlier step, and `data` of
+  // every block (None for a None).
+  py::class_<Holding>(m, "Holding")
+      .def(py::init<const py::list &>(), py::arg("blocks"))
+      .def("same", &Holding::Same, py::arg("blocks"));
+  m.def("storages", [](const py::list &blocks) {
+    py::list out(blocks.size());
+    for (size_t i = 0; i < blocks.size(); ++i) {
+      const py::handle b = blocks[i];
+      out[i] = b.is_none() ? py::none() : b.cast<PyBlock &>().get();
+    }
+    return out;
+  });
 
   py::enum_<BlockType>(m, "BlockType")
       .value("kUnknown", BlockType::kUnknown)

@@ -453,7 +453,7 @@ class Adam(_Adaptive):
 _core = operator.attrgetter("data")
 _dtype = operator.attrgetter("dtype")
 _place = operator.attrgetter("device")
-_storage_of = operator.attrgetter("data._block.data")
+_block_of = operator.attrgetter("data._block")
 
 
 def _same(a, b):
@@ -598,7 +598,7 @@ class AdamW(Optimizer):
             if not (_same(group.params, list(map(_core, params))) and
                     all([_same(column, list(map(table.get, keys)))
                          for table, column in zip(tables, columns)]) and
-                    _same(group.storage, list(map(_storage_of, itertools.chain(
+                    group.holding.same(list(map(_block_of, itertools.chain(
                         params, *columns))))):
                 found = None
         if found is None:

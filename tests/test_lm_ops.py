@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import test_dist
-from singa_amd import autograd, device, layer, model, opt, singa_wrap, tensor
+from singa_amd import _rt, autograd, device, layer, model, opt, singa_wrap, tensor
 from singa_amd.utils import checkpoint
 
 E32 = 2.0 ** -24
@@ -1482,3 +1482,44 @@ def test_adamw_two_ranks(cpu_dev, bits, use_graph):
     if bits == 32:
         for k, v in _ranks_step(0, 1, None, bits, use_graph).items():
             assert np.abs(v - res[0][k]).max() < 1e-5
+
+
+def test_blocks_and_their_storage_are_recognised(cpu_dev):
+    """The native list of an optimizer's blocks tells every change of one."""
+    cores = [put(cpu_dev, normal(i, 5)).data for i in range(3)]
+    blocks = [c._block for c in cores]
+    stored = _rt.storages(blocks + [None])
+    assert stored[3] is None
+    assert all(s is c._storage() for s, c in zip(stored, cores))
+    held = _rt.Holding(blocks)
+    assert held.same(list(blocks))
+    assert not held.same(blocks[:2]) and not held.same(blocks + blocks[:1])
+    assert not held.same([blocks[1], blocks[0], blocks[2]])
+    assert not held.same([None] * 3)
+    # another tensor in the block's place, the old one back, none
+    was = blocks[1].data
+    blocks[1].data = was.clone()
+    assert not held.same(blocks)
+    blocks[1].data = was
+    assert held.same(blocks)
+    blocks[1].free_data()
+    assert not held.same(blocks) and _rt.storages(blocks)[1] is None
+    # the blocks live as long as they are held
+    alone = _rt.Holding([cpu_dev.NewBlock(8)])
+    gc.collect()
+    assert not alone.same(blocks[:1])
+    with pytest.raises((RuntimeError, TypeError)):
+        _rt.Holding([1])
+    with pytest.raises((RuntimeError, TypeError)):
+        _rt.storages(["block"])
+
+
+def test_adamw_gradient_that_was_never_written(dev):
+    """Allocated on first use, as by every operator."""
+    for bits in (32, 8):
+        o, p = opt.AdamW(lr=0.1, weight_decay=0.0, state_bits=bits), put(
+            dev, normal(1, 300))
+        g = tensor.Tensor((300,), dev)
+        assert g.data._block.data is None
+        o.apply_many([(p, g)])
+        assert g.data._block.data is not None
